@@ -118,13 +118,18 @@ def work(case):
 # ---------------------------------------------------------------------------
 # inputs
 # ---------------------------------------------------------------------------
+def _power(e, bits, bias, whole, real):
+    """2^e for integers e of a type's normal range, exactly: the exponent field alone."""
+    return ((e.to(whole) + bias) << bits).view(real)
+
+
 def _planar(x, fmt):
     """The planar microscaled tensor of x [rows][k], by comparisons and the type's own rounding."""
     rows, k = x.shape
     b = x.float().reshape(rows, k // 32, 32)
     top = b.abs().amax(-1)
     byte = (top.view(torch.int32) >> 23).sub(EMAX[fmt]).clamp(0, 254)
-    v = torch.ldexp(b, (127 - byte).unsqueeze(-1)).reshape(rows, k)
+    v = (b * _power(127 - byte, 23, 127, torch.int32, torch.float32).unsqueeze(-1)).reshape(rows, k)
     if fmt == "mx8":
         codes = v.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8).reshape(-1)
     else:
@@ -149,8 +154,9 @@ def _values(planar, fmt, rows, k):
         half = torch.tensor(E2M1, device=planar.device)
         table = torch.cat([half, -half])
         e = torch.stack([table[(planar[:n] & 15).int()], table[(planar[:n] >> 4).int()]], -1)
-    scale = (planar[n:].int() - 127).reshape(-1, 1)
-    return torch.ldexp(e.reshape(-1, 32), scale).reshape(rows, k)
+    byte = planar[n:].int().reshape(-1, 1)
+    scale = torch.where(byte > 0, byte << 23, 1 << 22).view(torch.float32)  # 2^(byte - 127), at byte 0 a subnormal
+    return (e.reshape(-1, 32) * scale).reshape(rows, k)
 
 
 def prepare(case, seed):
@@ -245,6 +251,11 @@ def _run_own(s, case):
 # ---------------------------------------------------------------------------
 # the definition in 64 bits
 # ---------------------------------------------------------------------------
+def _times(x, e):
+    """x 2^e in 64 bits, exactly."""
+    return x * _power(e, 52, 1023, torch.int64, torch.float64)
+
+
 def _grid(x, fmt):
     """The values that the microscaled form of x [rows][k] (float64) stands for: each block's exponent is that of its
     largest magnitude less the element's, each element a multiple of its own spacing, rounded half to even."""
@@ -253,12 +264,12 @@ def _grid(x, fmt):
     _, e = torch.frexp(b.abs().amax(-1, keepdim=True))          # |x| in [2^(e-1), 2^e)
     shared = torch.clamp(e - 1 - EMAX[fmt], min=-127)
     shared = torch.where(b.abs().amax(-1, keepdim=True) == 0, torch.full_like(shared, -127), shared)
-    v = torch.ldexp(b, -shared)
+    v = _times(b, -shared)
     mantissa, lowest = (3, -6) if fmt == "mx8" else (1, 0)
     _, ev = torch.frexp(v)
     spacing = torch.clamp(ev - 1, min=lowest) - mantissa
-    q = torch.ldexp(torch.round(torch.ldexp(v, -spacing)), spacing).clamp(-LARGEST[fmt], LARGEST[fmt])
-    return torch.ldexp(q, shared).reshape(rows, k)
+    q = _times(torch.round(_times(v, -spacing)), spacing).clamp(-LARGEST[fmt], LARGEST[fmt])
+    return _times(q, shared).reshape(rows, k)
 
 
 def _decode(planar, fmt, rows, k):
@@ -272,9 +283,9 @@ def _decode(planar, fmt, rows, k):
         c = torch.stack([p & 15, p >> 4], -1).reshape(-1)
         sign, e, f, bias, bits = c >> 3, (c >> 1) & 3, c & 1, 1, 1
     whole = torch.where(e > 0, f + (1 << bits), f).double()
-    v = torch.ldexp(whole, torch.clamp(e, min=1) - bias - bits) * (1 - 2 * sign).double()
+    v = _times(whole, torch.clamp(e, min=1) - bias - bits) * (1 - 2 * sign).double()
     x = planar[n:].to(torch.int32).reshape(-1, 1) - 127
-    return torch.ldexp(v.reshape(-1, 32), x).reshape(rows, k)
+    return _times(v.reshape(-1, 32), x).reshape(rows, k)
 
 
 def exact(case, seed):
