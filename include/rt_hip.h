@@ -123,6 +123,7 @@ size_t rt_gemm_workspace_held(void *stream);
 #define RT_LINEAR_F32 3    /* f32 [rows][cols] */
 #define RT_LINEAR_Q6K 4    /* planar Q6_K (rt_q6k_repack) */
 #define RT_LINEAR_Q8_0 5   /* planar Q8_0 (rt_q8_0_repack) */
+#define RT_LINEAR_MXFP4 6  /* planar MXFP4 (rt_mx_quantize) */
 
 /* ---------------------------------------------------------------------------
  * Q6_K and Q8_0 weights kept packed on the device.  No counterpart in the
@@ -178,6 +179,78 @@ rt_status rt_q8_0_dequant_f32(const void *w, size_t n_elem, float *out, void *st
  * weights; device pointers, w and x 16-byte aligned. */
 rt_status rt_q6k_gemv(const void *w, const float *x, float *y, int64_t n, int64_t k, void *stream);
 rt_status rt_q8_0_gemv(const void *w, const float *x, float *y, int64_t n, int64_t k, void *stream);
+/* ---------------------------------------------------------------------------
+ * Microscaled tensors (OCP MX v1.0): blocks of 32 along k share a power-of-two
+ * scale.  No counterpart in the reference; they are the 4- and 8-bit formats
+ * that the CDNA4 matrix cores multiply as they lie in memory.  Planar, like
+ * Q8_0 here: the elements of [rows][k], then one e8m0 byte per block,
+ * [rows][k/32] (byte b is 2^(b-127), 255 NaN); k % 32 == 0.
+ *   RT_MX_FP8: e4m3 bytes, rows*k + rows*k/32 bytes in all
+ *   RT_MX_FP4: e2m1 codes, two to a byte, the even element in the low four
+ *              bits, rows*k/2 + rows*k/32 bytes; a weight in this form is
+ *              RT_LINEAR_MXFP4
+ * ------------------------------------------------------------------------- */
+#define RT_MX_FP4 4
+#define RT_MX_FP8 8
+/* Types of ordinary arrays in the calls below. */
+#define RT_TYPE_F32 0
+#define RT_TYPE_BF16 1
+/* Bytes of a microscaled [rows][k] tensor (0 for a bad format or k). */
+size_t rt_mx_bytes(int32_t fmt, int64_t rows, int64_t k);
+/* Quantises x [rows][k] (RT_TYPE_*): a block's scale is the exponent of its
+ * largest magnitude less the element type's (8 for e4m3, 2 for e2m1), elements
+ * are rounded to nearest even and saturated (448, 6), the conversion of the
+ * standard's section 6.3.  A block that holds an infinity or a NaN becomes 32
+ * NaN (scale 255).  Device pointers, 16-byte aligned; weights at load time and
+ * activations alike; rows = 0 is no work. */
+rt_status rt_mx_quantize(int32_t x_type, const void *x, int32_t fmt, void *out, int64_t rows, int64_t k,
+                         void *stream);
+/* The values of a microscaled tensor, f32 (exact) or bf16 (exact, but for
+ * subnormals of bf16). */
+rt_status rt_mx_dequantize(int32_t fmt, const void *src, int32_t out_type, void *out, int64_t rows, int64_t k,
+                           void *stream);
+/* RMSNorm with the residual's addition, the result microscaled:
+ *   u = x, or x / rms(x) * (1 + post_gamma) where post_gamma is not NULL
+ *   h = residual + u                        (h = u where residual is NULL)
+ *   out = MX(h / rms(h) * (1 + gamma)),     rms(v) = sqrt(mean(v^2) + eps)
+ * per row of k (k % 32 == 0, k <= 32768): the step between two Gemma-3
+ * sublayers (post-norm of the one, residual, pre-norm of the other).  sum_out
+ * (f32 [rows][k], may be NULL) receives h, and may be the residual's or an f32
+ * x's own buffer, whole; no other buffers may overlap.  x is f32 or bf16, the rest f32; device
+ * pointers, 16-byte aligned.  The row is computed in 64 bits, h rounded
+ * once to f32 and the result once to its element. */
+rt_status rt_add_rmsnorm_mx(int32_t x_type, const void *x, const float *residual, const float *post_gamma,
+                            const float *gamma, float eps, int32_t fmt, void *out, float *sum_out, int64_t rows,
+                            int64_t k, void *stream);
+/* out = MX(gelu_tanh(gate) * up), the gated activation of a Gemma-3
+ * feed-forward, row r of gate and up at + r*ld elements (ld >= k, whole 16
+ * bytes: the two halves of a fused gate|up product are ld = 2k apart per row
+ * with up = gate + k).  gate and up have the type RT_TYPE_*; device pointers,
+ * 16-byte aligned. */
+rt_status rt_gelu_mul_mx(int32_t type, const void *gate, const void *up, int64_t ld, int32_t fmt, void *out,
+                         int64_t rows, int64_t k, void *stream);
+/* c[m][n] = a[m][k] . W[n][k] (+ bias[n], f32, or NULL): a microscaled
+ * (RT_MX_FP8 or RT_MX_FP4), W RT_LINEAR_MXFP4, c f32 or bf16 (c_type), on the
+ * scaled matrix instructions with f32 accumulation: c carries the sum's
+ * rounding alone, but that an MXFP8 product into bf16 may lose terms below
+ * 2^-13 of the largest of their eight neighbours in k (5e-6 of c's norm).  k % 32 == 0; a and w 16-byte aligned.
+ * Workspace of rt_q4k_gemm_f32: up to (m + n) * k / 32 bytes, plus split-K
+ * partials. */
+rt_status rt_mx_gemm(int32_t a_fmt, const void *a, const void *w, const float *bias, int32_t c_type, void *c,
+                     int64_t m, int64_t n, int64_t k, void *stream);
+/* c[m][n] = a[m][k] . W[n][k] with activations in f32 or bf16 (a_type) on an
+ * RT_LINEAR_MXFP4 weight, f32 out.  The activations run as e4m3 digit planes
+ * (five hold an f32, three a bf16, down to 2^-30 and 2^-20 of the largest value
+ * in their block of 32), so c is exact up to the f32 sum; a row with an
+ * infinity or a NaN gives a row of NaN.  rt_linear_gemm_f32,
+ * rt_qlinear_forward and rt_linear_gemv_batch take RT_LINEAR_MXFP4 the same
+ * way.  k % 32 == 0; a and w 16-byte aligned.  Workspace: as rt_mx_gemm, plus
+ * five (three) bytes per element of a. */
+rt_status rt_mxfp4_gemm(int32_t a_type, const void *a, const void *w, float *c, int64_t m, int64_t n, int64_t k,
+                        void *stream);
+/* y[n] = W[n,k] . x[k] on an RT_LINEAR_MXFP4 weight, x and y f32. */
+rt_status rt_mxfp4_gemv(const void *w, const float *x, float *y, int64_t n, int64_t k, void *stream);
+
 /* c[m][n] = a[m][k] . W[n][k] for a weight in any RT_LINEAR_* format (Q6_K
  * and Q8_0 planar): the matmul of QLinear::forward (qlinear.rs:82-111).
  * Replaces matmul_q4k_t_exact for RT_LINEAR_Q4K (as rt_q4k_gemm_f32),

@@ -29,7 +29,9 @@ LIB_PATH = pathlib.Path(os.environ["RT_HIP_LIB"]).resolve() if os.environ.get("R
 RT_OK, RT_EINVAL, RT_EHIP, RT_ENOMEM, RT_ESTATE = 0, 1, 2, 3, 4
 
 
-LINEAR_Q4K, LINEAR_BF16, LINEAR_F32, LINEAR_Q6K, LINEAR_Q8_0 = 1, 2, 3, 4, 5  # RT_LINEAR_* (rt_hip.h)
+LINEAR_Q4K, LINEAR_BF16, LINEAR_F32, LINEAR_Q6K, LINEAR_Q8_0, LINEAR_MXFP4 = 1, 2, 3, 4, 5, 6  # RT_LINEAR_* (rt_hip.h)
+MX_FP4, MX_FP8 = 4, 8  # RT_MX_*
+TYPE_F32, TYPE_BF16 = 0, 1  # RT_TYPE_*
 
 
 class RtError(RuntimeError):
@@ -79,6 +81,14 @@ _SIGNATURES = {
     "rt_q6k_gemv": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),
     "rt_q8_0_gemv": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),
     "rt_linear_gemm_f32": (_i32, [_i32, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "rt_mx_bytes": (_sz, [_i32, _i64, _i64]),
+    "rt_mx_quantize": (_i32, [_i32, _vp, _i32, _vp, _i64, _i64, _vp]),
+    "rt_mx_dequantize": (_i32, [_i32, _vp, _i32, _vp, _i64, _i64, _vp]),
+    "rt_add_rmsnorm_mx": (_i32, [_i32, _vp, _vp, _vp, _vp, C.c_float, _i32, _vp, _vp, _i64, _i64, _vp]),
+    "rt_gelu_mul_mx": (_i32, [_i32, _vp, _vp, _i64, _i32, _vp, _i64, _i64, _vp]),
+    "rt_mx_gemm": (_i32, [_i32, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp]),
+    "rt_mxfp4_gemm": (_i32, [_i32, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "rt_mxfp4_gemv": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),
     "rt_q4k_gemv_multi": (_i32, [_vp, _vp, _vp, _i32, _vp, _i64, _vp]),
     "rt_q4k_gemm_bf16": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "rt_q4k_gemm_f32": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _vp]),
@@ -243,6 +253,68 @@ def q6k_gemv(w, x, y, n: int, k: int, stream=None) -> None:
 def q8_0_gemv(w, x, y, n: int, k: int, stream=None) -> None:
     """y = W x on planar Q8_0 weights (q8_0_repack)."""
     check(lib().rt_q8_0_gemv(_p(w), _p(x), _p(y), n, k, _stream(stream)))
+
+
+def _type(t) -> int:
+    """RT_TYPE_* of a torch tensor."""
+    import torch
+    if t.dtype is torch.float32:
+        return TYPE_F32
+    if t.dtype is torch.bfloat16:
+        return TYPE_BF16
+    raise TypeError(f"float32 or bfloat16 wanted, got {t.dtype}")
+
+
+def mx_bytes(fmt: int, rows: int, k: int) -> int:
+    """Bytes of a planar microscaled [rows][k] tensor (fmt MX_FP8 or MX_FP4)."""
+    return int(lib().rt_mx_bytes(fmt, rows, k))
+
+
+def mx_quantize(x, fmt: int, out, rows: int, k: int, stream=None) -> None:
+    """out = MX(x), x [rows][k] float32 or bfloat16, out mx_bytes(fmt, rows, k)
+    bytes: elements, then the e8m0 scales of their blocks of 32.  An MXFP4
+    weight made so is a LINEAR_MXFP4 one."""
+    check(lib().rt_mx_quantize(_type(x), _p(x), fmt, _p(out), rows, k, _stream(stream)))
+
+
+def mx_dequantize(fmt: int, src, out, rows: int, k: int, stream=None) -> None:
+    """The values of a microscaled tensor, into a float32 or bfloat16 out."""
+    check(lib().rt_mx_dequantize(fmt, _p(src), _type(out), _p(out), rows, k, _stream(stream)))
+
+
+def add_rmsnorm_mx(x, gamma, eps: float, fmt: int, out, rows: int, k: int, residual=None, post_gamma=None,
+                   sum_out=None, stream=None) -> None:
+    """h = residual + x (x first normed with post_gamma, if given), out =
+    MX(h / rms(h) * (1 + gamma)), sum_out = h: the step between two Gemma-3
+    sublayers.  sum_out may be residual, or a float32 x."""
+    check(lib().rt_add_rmsnorm_mx(_type(x), _p(x), _p(residual), _p(post_gamma), _p(gamma), eps, fmt, _p(out),
+                                  _p(sum_out), rows, k, _stream(stream)))
+
+
+def gelu_mul_mx(gate, up, fmt: int, out, rows: int, k: int, ld: int | None = None, stream=None) -> None:
+    """out = MX(gelu_tanh(gate) * up), row r of both at r * ld elements
+    (default k; 2 k for the halves of a fused gate|up product)."""
+    ty = _type(gate)
+    if _type(up) != ty:
+        raise TypeError(f"gate and up must have the same type, got {gate.dtype} and {up.dtype}")
+    check(lib().rt_gelu_mul_mx(ty, _p(gate), _p(up), k if ld is None else ld, fmt, _p(out), rows, k, _stream(stream)))
+
+
+def mx_gemm(a_fmt: int, a, w, c, m: int, n: int, k: int, bias=None, stream=None) -> None:
+    """c[m][n] = a[m][k] . W[n][k] (+ bias[n]): a microscaled (MX_FP8 or
+    MX_FP4), W a LINEAR_MXFP4 weight, c float32 or bfloat16."""
+    check(lib().rt_mx_gemm(a_fmt, _p(a), _p(w), _p(bias), _type(c), _p(c), m, n, k, _stream(stream)))
+
+
+def mxfp4_gemm(a, w, c, m: int, n: int, k: int, stream=None) -> None:
+    """c[m][n] = a[m][k] . W[n][k]: a float32 or bfloat16, W a LINEAR_MXFP4
+    weight, c float32; the activations keep their bits."""
+    check(lib().rt_mxfp4_gemm(_type(a), _p(a), _p(w), _p(c), m, n, k, _stream(stream)))
+
+
+def mxfp4_gemv(w, x, y, n: int, k: int, stream=None) -> None:
+    """y = W x on a LINEAR_MXFP4 weight (mx_quantize), x and y float32."""
+    check(lib().rt_mxfp4_gemv(_p(w), _p(x), _p(y), n, k, _stream(stream)))
 
 
 def q4k_gemv_multi(ws, ys, ns, x, k: int, stream=None) -> None:

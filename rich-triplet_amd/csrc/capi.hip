@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "../../include/rt_hip.h"
+#include "mx_kernels.hpp"
 #include "rt_capi_util.hpp"
 #include "q4k_gemv_mb.hpp"
 #include "rt_kernels.hpp"
@@ -160,8 +161,6 @@ rt_status rt_q8_0_gemv(const void *w, const float *x, float *y, int64_t n, int64
 }  // extern "C"
 
 namespace {
-rt_status gemm_workspace(size_t bytes, hipStream_t stream, void **out);
-
 rt_status q4k_gemm_entry(const char *who, const void *a, bool a_bf16, const void *w, const float *bias, float *c,
                          int64_t m, int64_t n, int64_t k, void *stream) {
   if (m <= 0 || n <= 0 || k <= 0)
@@ -212,7 +211,7 @@ static rt_status linear_forward(const char *who, int32_t fmt, const void *w, con
                                 float *c, int64_t m, int64_t n, int64_t k, void *stream) {
   hipStream_t s = (hipStream_t)stream;
   if (fmt != RT_LINEAR_Q4K && fmt != RT_LINEAR_BF16 && fmt != RT_LINEAR_Q6K && fmt != RT_LINEAR_Q8_0 &&
-      fmt != RT_LINEAR_F32)
+      fmt != RT_LINEAR_F32 && fmt != RT_LINEAR_MXFP4)
     return set_error(RT_EINVAL, "%s: unsupported format %d", who, fmt);
   if (m <= 0 || n <= 0 || k <= 0)
     return set_error(RT_EINVAL, "%s: m=%lld n=%lld k=%lld must be positive", who, (long long)m, (long long)n,
@@ -223,6 +222,7 @@ static rt_status linear_forward(const char *who, int32_t fmt, const void *w, con
   const int align = (fmt == RT_LINEAR_Q4K || fmt == RT_LINEAR_Q6K) ? 256
                     : fmt == RT_LINEAR_F32                         ? 4
                     : fmt == RT_LINEAR_BF16 && (few || k % 64)     ? 8
+                    : fmt == RT_LINEAR_MXFP4                       ? 32
                                                                    : 64;
   if (k % align != 0) return set_error(RT_EINVAL, "%s: k=%lld must be a multiple of %d", who, (long long)k, align);
   if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return set_error(RT_EINVAL, "%s: m, n or k exceeds int32", who);
@@ -239,6 +239,8 @@ static rt_status linear_forward(const char *who, int32_t fmt, const void *w, con
   if (fmt == RT_LINEAR_BF16 && (few || k % 64 != 0))
     return hip_error(launch_bf16_gemv_rows(static_cast<const uint16_t *>(w), a, bias, c, (int)m, (int)n, (int)k, s),
                      who);
+  if (fmt == RT_LINEAR_MXFP4)  // f32 activations as e4m3 digits, the weight as stored
+    return mx_product(who, kMxActF32, a, w, bias, c, false, m, n, k, s);
   const bool rows = rows_gemm_ok(fmt, (int)m, (int)n, (int)k);
   void *ws = nullptr;
   rt_status st = gemm_workspace(rows ? rows_gemm_workspace_bytes(fmt, (int)m, (int)n, (int)k)
@@ -282,11 +284,12 @@ rt_status rt_linear_gemv_batch(int32_t fmt, const void *w, const float *a, float
                                void *stream) {
   static const char *who = "rt_linear_gemv_batch";
   if (fmt == RT_LINEAR_Q4K) return rt_q4k_gemv_batch(w, a, c, m, n, k, stream);
-  if (fmt != RT_LINEAR_Q6K && fmt != RT_LINEAR_Q8_0 && fmt != RT_LINEAR_BF16)
+  if (fmt != RT_LINEAR_Q6K && fmt != RT_LINEAR_Q8_0 && fmt != RT_LINEAR_BF16 && fmt != RT_LINEAR_MXFP4)
     return set_error(RT_EINVAL, "%s: format %d has no batched GEMV", who, fmt);
-  rt_status st = check_gemv_shape(who, w, a, c, n, k, fmt == RT_LINEAR_Q6K ? 256 : 64);
+  rt_status st = check_gemv_shape(who, w, a, c, n, k, fmt == RT_LINEAR_Q6K ? 256 : fmt == RT_LINEAR_MXFP4 ? 32 : 64);
   if (st != RT_OK) return st;
   if (m < 1 || m > kMbMaxRows) return set_error(RT_EINVAL, "%s: m=%lld outside [1, 8]", who, (long long)m);
+  if (fmt == RT_LINEAR_MXFP4) return mx_product(who, kMxActF32, a, w, nullptr, c, false, m, n, k, (hipStream_t)stream);
   const size_t stage = fmt == RT_LINEAR_BF16 ? 0 : (mb_stage_bytes((int)k) + 255) & ~size_t(255);
   void *ws = nullptr;
   st = gemm_workspace(std::max<size_t>(stage + kquant_mb_part_bytes((int)n, (int)k), 256), (hipStream_t)stream, &ws);
@@ -444,8 +447,9 @@ struct GemmWorkspace {
   size_t retired_bytes = 0;
 };
 thread_local std::map<std::pair<int, hipStream_t>, GemmWorkspace> g_gemm_ws;
+}  // namespace
 
-rt_status gemm_workspace(size_t bytes, hipStream_t stream, void **out) {
+rt_status rt::gemm_workspace(size_t bytes, hipStream_t stream, void **out) {
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return hip_error(e, "hipGetDevice");
@@ -471,6 +475,7 @@ rt_status gemm_workspace(size_t bytes, hipStream_t stream, void **out) {
   return RT_OK;
 }
 
+namespace {
 template <typename LaunchFn>
 rt_status host_gemv(const char *who, const float *a, size_t k, const void *w_host, size_t w_bytes, size_t rows,
                     float *out, LaunchFn launch) {

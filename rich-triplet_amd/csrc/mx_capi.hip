@@ -1,0 +1,138 @@
+// mx_capi.hip -- extern "C" entry points of the microscaled operators (declared
+// in include/rt_hip.h): every shape, pointer and format the kernels assume is
+// checked here, on the host.
+#include <hip/hip_runtime.h>
+
+#include "../../include/rt_hip.h"
+#include "mx_common.hpp"
+#include "mx_kernels.hpp"
+#include "rt_capi_util.hpp"
+
+using namespace rt;
+
+static_assert(RT_MX_FP4 == kMxFp4 && RT_MX_FP8 == kMxFp8, "formats are their elements' bits");
+
+namespace {
+
+rt_status check_mx(const char *who, int32_t fmt, int32_t type, int64_t rows, int64_t k) {
+  if (fmt != RT_MX_FP4 && fmt != RT_MX_FP8) return set_error(RT_EINVAL, "%s: format %d is neither RT_MX_FP4 nor RT_MX_FP8", who, fmt);
+  if (type != RT_TYPE_F32 && type != RT_TYPE_BF16) return set_error(RT_EINVAL, "%s: type %d is neither RT_TYPE_F32 nor RT_TYPE_BF16", who, type);
+  if (rows < 0 || k <= 0) return set_error(RT_EINVAL, "%s: rows=%lld must not be negative, k=%lld must be positive", who, (long long)rows, (long long)k);
+  if (k % kMxBlock != 0) return set_error(RT_EINVAL, "%s: k=%lld must be a multiple of 32", who, (long long)k);
+  if (k > INT32_MAX || rows > (int64_t(1) << 48) / k)
+    return set_error(RT_EINVAL, "%s: rows=%lld k=%lld is too large", who, (long long)rows, (long long)k);
+  return RT_OK;
+}
+
+rt_status check_product(const char *who, const void *a, const void *w, const float *bias, const void *c, bool c_bf16,
+                        int64_t m, int64_t n, int64_t k) {
+  if (m <= 0 || n <= 0 || k <= 0)
+    return set_error(RT_EINVAL, "%s: m=%lld n=%lld k=%lld must be positive", who, (long long)m, (long long)n, (long long)k);
+  if (k % kMxBlock != 0) return set_error(RT_EINVAL, "%s: k=%lld must be a multiple of 32", who, (long long)k);
+  if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return set_error(RT_EINVAL, "%s: m, n or k exceeds int32", who);
+  if (!a || !w || !c) return set_error(RT_EINVAL, "%s: null pointer", who);
+  if (!aligned16(a) || !aligned16(w)) return set_error(RT_EINVAL, "%s: a and w must be 16-byte aligned", who);
+  if ((reinterpret_cast<uintptr_t>(c) & (c_bf16 ? 1u : 3u)) != 0)
+    return set_error(RT_EINVAL, "%s: c must be aligned to its elements", who);
+  if (bias && (reinterpret_cast<uintptr_t>(bias) & 3u) != 0) return set_error(RT_EINVAL, "%s: bias must be 4-byte aligned", who);
+  return RT_OK;
+}
+
+}  // namespace
+
+rt_status rt::mx_product(const char *who, int act, const void *a, const void *w, const float *bias, void *c,
+                         bool c_bf16, int64_t m, int64_t n, int64_t k, hipStream_t s) {
+  const size_t need = mx_gemm_workspace_bytes((MxAct)act, (int)m, (int)n, (int)k);
+  void *ws = nullptr;
+  if (need) {
+    rt_status st = gemm_workspace(need, s, &ws);
+    if (st != RT_OK) return st;
+  }
+  return hip_error(launch_mx_gemm((MxAct)act, a, w, bias, c, c_bf16, (int)m, (int)n, (int)k, ws, s), who);
+}
+
+extern "C" {
+
+size_t rt_mx_bytes(int32_t fmt, int64_t rows, int64_t k) {
+  if ((fmt != RT_MX_FP4 && fmt != RT_MX_FP8) || rows <= 0 || k <= 0 || k % kMxBlock != 0) return 0;
+  const size_t n = (size_t)rows * (size_t)k;
+  return mx_elem_bytes(fmt, n) + n / kMxBlock;
+}
+
+rt_status rt_mx_quantize(int32_t x_type, const void *x, int32_t fmt, void *out, int64_t rows, int64_t k, void *stream) {
+  static const char *who = "rt_mx_quantize";
+  rt_status st = check_mx(who, fmt, x_type, rows, k);
+  if (st != RT_OK || rows == 0) return st;
+  if (!x || !out) return set_error(RT_EINVAL, "%s: null pointer", who);
+  if (!aligned16(x) || !aligned16(out)) return set_error(RT_EINVAL, "%s: buffers must be 16-byte aligned", who);
+  return hip_error(launch_mx_quantize(fmt, x, x_type == RT_TYPE_BF16, out, (size_t)rows * (size_t)k, (hipStream_t)stream), who);
+}
+
+rt_status rt_mx_dequantize(int32_t fmt, const void *src, int32_t out_type, void *out, int64_t rows, int64_t k, void *stream) {
+  static const char *who = "rt_mx_dequantize";
+  rt_status st = check_mx(who, fmt, out_type, rows, k);
+  if (st != RT_OK || rows == 0) return st;
+  if (!src || !out) return set_error(RT_EINVAL, "%s: null pointer", who);
+  if (!aligned16(src) || !aligned16(out)) return set_error(RT_EINVAL, "%s: buffers must be 16-byte aligned", who);
+  return hip_error(launch_mx_dequantize(fmt, src, out, out_type == RT_TYPE_BF16, (size_t)rows * (size_t)k, (hipStream_t)stream), who);
+}
+
+rt_status rt_add_rmsnorm_mx(int32_t x_type, const void *x, const float *residual, const float *post_gamma,
+                            const float *gamma, float eps, int32_t fmt, void *out, float *sum_out, int64_t rows,
+                            int64_t k, void *stream) {
+  static const char *who = "rt_add_rmsnorm_mx";
+  rt_status st = check_mx(who, fmt, x_type, rows, k);
+  if (st != RT_OK) return st;
+  if (k > kNormMaxK) return set_error(RT_EINVAL, "%s: k=%lld exceeds %d", who, (long long)k, kNormMaxK);
+  if (!(eps >= 0.f)) return set_error(RT_EINVAL, "%s: eps=%g must not be negative", who, (double)eps);
+  if (rows == 0) return RT_OK;
+  if (!x || !gamma || !out) return set_error(RT_EINVAL, "%s: null pointer", who);
+  if (!aligned16(x) || !aligned16(residual) || !aligned16(post_gamma) || !aligned16(gamma) || !aligned16(out) || !aligned16(sum_out))
+    return set_error(RT_EINVAL, "%s: buffers must be 16-byte aligned", who);
+  if (x_type == RT_TYPE_BF16 && (const void *)sum_out == x)
+    return set_error(RT_EINVAL, "%s: sum_out (f32) cannot be a bf16 x's buffer", who);
+  return hip_error(launch_add_rmsnorm_mx(fmt, x, x_type == RT_TYPE_BF16, residual, post_gamma, gamma, eps, out, sum_out,
+                                         (size_t)rows, (int)k, (hipStream_t)stream), who);
+}
+
+rt_status rt_gelu_mul_mx(int32_t type, const void *gate, const void *up, int64_t ld, int32_t fmt, void *out,
+                         int64_t rows, int64_t k, void *stream) {
+  static const char *who = "rt_gelu_mul_mx";
+  rt_status st = check_mx(who, fmt, type, rows, k);
+  if (st != RT_OK) return st;
+  const int64_t unit = type == RT_TYPE_BF16 ? 8 : 4;
+  if (ld < k || ld % unit != 0 || ld > (int64_t(1) << 40))
+    return set_error(RT_EINVAL, "%s: ld=%lld must be at least k=%lld and whole 16 bytes", who, (long long)ld, (long long)k);
+  if (rows == 0) return RT_OK;
+  if (!gate || !up || !out) return set_error(RT_EINVAL, "%s: null pointer", who);
+  if (!aligned16(gate) || !aligned16(up) || !aligned16(out)) return set_error(RT_EINVAL, "%s: buffers must be 16-byte aligned", who);
+  return hip_error(launch_gelu_mul_mx(fmt, gate, up, type == RT_TYPE_BF16, (size_t)ld, out, (size_t)rows, (int)k, (hipStream_t)stream), who);
+}
+
+rt_status rt_mx_gemm(int32_t a_fmt, const void *a, const void *w, const float *bias, int32_t c_type, void *c, int64_t m,
+                     int64_t n, int64_t k, void *stream) {
+  static const char *who = "rt_mx_gemm";
+  if (a_fmt != RT_MX_FP4 && a_fmt != RT_MX_FP8) return set_error(RT_EINVAL, "%s: format %d is neither RT_MX_FP4 nor RT_MX_FP8", who, a_fmt);
+  if (c_type != RT_TYPE_F32 && c_type != RT_TYPE_BF16) return set_error(RT_EINVAL, "%s: type %d is neither RT_TYPE_F32 nor RT_TYPE_BF16", who, c_type);
+  const bool bf16 = c_type == RT_TYPE_BF16;
+  rt_status st = check_product(who, a, w, bias, c, bf16, m, n, k);
+  if (st != RT_OK) return st;
+  return mx_product(who, a_fmt == RT_MX_FP8 ? kMxActFp8 : kMxActFp4, a, w, bias, c, bf16, m, n, k, (hipStream_t)stream);
+}
+
+rt_status rt_mxfp4_gemm(int32_t a_type, const void *a, const void *w, float *c, int64_t m, int64_t n, int64_t k, void *stream) {
+  static const char *who = "rt_mxfp4_gemm";
+  if (a_type != RT_TYPE_F32 && a_type != RT_TYPE_BF16) return set_error(RT_EINVAL, "%s: type %d is neither RT_TYPE_F32 nor RT_TYPE_BF16", who, a_type);
+  rt_status st = check_product(who, a, w, nullptr, c, false, m, n, k);
+  if (st != RT_OK) return st;
+  return mx_product(who, a_type == RT_TYPE_F32 ? kMxActF32 : kMxActBf16, a, w, nullptr, c, false, m, n, k, (hipStream_t)stream);
+}
+
+rt_status rt_mxfp4_gemv(const void *w, const float *x, float *y, int64_t n, int64_t k, void *stream) {
+  static const char *who = "rt_mxfp4_gemv";
+  rt_status st = check_product(who, x, w, nullptr, y, false, 1, n, k);
+  if (st != RT_OK) return st;
+  return mx_product(who, kMxActF32, x, w, nullptr, y, false, 1, n, k, (hipStream_t)stream);
+}
+
+}  // extern "C"

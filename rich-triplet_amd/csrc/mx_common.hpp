@@ -1,0 +1,115 @@
+// mx_common.hpp -- microscaled (OCP MX v1.0) tensors: planar layout, block
+// scales and the conversion of eight values held by one thread.
+//
+//   [rows][k] elements, then [rows][k/32] e8m0 scale bytes (byte b: 2^(b-127),
+//   255: NaN).  RT_MX_FP8: one e4m3 byte per element; RT_MX_FP4: e2m1 codes,
+//   two to a byte, the even element low.  k % 32 == 0, so the element plane is
+//   whole 16-byte units and a block never crosses a row.
+//
+// A block's scale is that of the standard's section 6.3: the exponent of its
+// largest magnitude less the element's largest exponent (8 for e4m3, 2 for
+// e2m1), held to 0..254; elements are x 2^(127-b) rounded to nearest even,
+// saturated at the largest element (448, 6).  A block with an infinity or a
+// NaN gets scale 255 and elements 0: it reads back as 32 NaN.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "rt_device.hpp"
+
+namespace rt {
+
+constexpr int kMxBlock = 32;
+constexpr int kMxFp4 = 4, kMxFp8 = 8;  // RT_MX_FP4, RT_MX_FP8: bits of an element
+
+__host__ __device__ inline size_t mx_elem_bytes(int fmt, size_t n) { return fmt == kMxFp8 ? n : n / 2; }
+
+// Scale byte of a block whose largest |x| has these f32 bits (as integers,
+// infinities and NaN order above every finite value).
+template <int FMT>
+RT_DEV uint32_t mx_scale_byte(uint32_t amax_bits) {
+  const int e = (int)(amax_bits >> 23), b = max(e - (FMT == kMxFp8 ? 8 : 2), 0);
+  return e == 255 ? 255u : (uint32_t)b;
+}
+// 2^(127-b) for b <= 254
+RT_DEV float mx_inv_scale(uint32_t b) { return bits_f32((254u - min(b, 253u)) << 23); }
+// 2^(b-127); NaN at 255
+RT_DEV float mx_scale(uint32_t b) { return bits_f32(b == 0 ? 0x00400000u : b == 255 ? 0x7FC00000u : b << 23); }
+
+// Largest |x| bits over the four lanes (aligned quad) that hold a block.
+RT_DEV uint32_t quad_max_u32(uint32_t v) {
+  v = max(v, dpp_u32<0xB1>(v));
+  return max(v, dpp_u32<0x4E>(v));
+}
+RT_DEV uint32_t absmax8_bits(const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, f32_bits(v[i]) & 0x7FFFFFFFu);
+  return m;
+}
+
+// Eight scaled values as codes: two dwords of e4m3 or one of e2m1.  The
+// conversions round to nearest even; e4m3 is saturated first (past 464 the
+// instruction gives NaN), e2m1 saturates in the instruction.
+RT_DEV uint2 fp8x8(const float (&v)[8]) {
+  float t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_fmed3f(v[i], -448.f, 448.f);
+  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(t[0], t[1], 0, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(t[2], t[3], lo, true);
+  int hi = __builtin_amdgcn_cvt_pk_fp8_f32(t[4], t[5], 0, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(t[6], t[7], hi, true);
+  return make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+RT_DEV uint32_t fp4x8(const float (&v)[8]) {
+  uint32_t r = 0;
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], 1.0f, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], 1.0f, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], 1.0f, 2);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], 1.0f, 3);
+  return r;
+}
+
+// Quantises group i8 (elements 8 i8 .. 8 i8 + 7 of a flat tensor): a block is
+// one aligned quad of lanes, all four of which call this together.
+template <int FMT>
+RT_DEV void mx_store8(const float (&v)[8], uint8_t *elems, uint8_t *scales, size_t i8) {
+  const uint32_t b = mx_scale_byte<FMT>(quad_max_u32(absmax8_bits(v)));
+  const float inv = b == 255 ? 0.f : mx_inv_scale(b);
+  float t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = v[i] * inv;
+  uint2 q;
+  if constexpr (FMT == kMxFp8) q = fp8x8(t);
+  else q.x = fp4x8(t);
+  if (b == 255) q = make_uint2(0, 0);  // inf * 0 is NaN
+  if constexpr (FMT == kMxFp8) reinterpret_cast<uint2 *>(elems)[i8] = q;
+  else reinterpret_cast<uint32_t *>(elems)[i8] = q.x;
+  if ((threadIdx.x & 3) == 0) scales[i8 >> 2] = (uint8_t)b;
+}
+
+// Eight consecutive f32 or bf16 values.
+RT_DEV void load8(const float *p, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+RT_DEV void load8(const uint16_t *p, float (&v)[8]) {
+  const uint4 a = *reinterpret_cast<const uint4 *>(p);
+  v[0] = bf16_lo(a.x), v[1] = bf16_hi(a.x), v[2] = bf16_lo(a.y), v[3] = bf16_hi(a.y);
+  v[4] = bf16_lo(a.z), v[5] = bf16_hi(a.z), v[6] = bf16_lo(a.w), v[7] = bf16_hi(a.w);
+}
+RT_DEV void store8(float *p, const float (&v)[8]) {
+  reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+RT_DEV uint32_t bf16_pair(float lo, float hi) {
+  return (uint32_t)f32_to_bf16_bits(lo) | ((uint32_t)f32_to_bf16_bits(hi) << 16);
+}
+RT_DEV void store8(uint16_t *p, const float (&v)[8]) {
+  *reinterpret_cast<uint4 *>(p) =
+      make_uint4(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7]));
+}
+
+}  // namespace rt

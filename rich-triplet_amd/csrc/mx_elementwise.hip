@@ -1,0 +1,262 @@
+// mx_elementwise.hip -- conversion to and from microscaled tensors, and the
+// two producers that end in one: RMSNorm with the residual's addition, and the
+// gated GELU.
+//
+// Every kernel gives a thread eight consecutive elements, so a block of 32 is
+// one aligned quad of lanes (two DPP maxima) and every load and store is 4 to
+// 32 bytes.  All of them are bound by memory: one read of each input, one write
+// of each output.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "mx_common.hpp"
+#include "mx_kernels.hpp"
+#include "rt_device.hpp"
+
+namespace rt {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxGrid = 1 << 16;
+
+template <int FMT, class T>
+__global__ __launch_bounds__(kThreads) void k_mx_quantize(const T *__restrict__ x, uint8_t *__restrict__ elems,
+                                                          uint8_t *__restrict__ scales, size_t n8) {
+  // n8 is a multiple of 4, so a quad is in or out as a whole
+  for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < n8; i += (size_t)gridDim.x * kThreads) {
+    float v[8];
+    load8(x + 8 * i, v);
+    mx_store8<FMT>(v, elems, scales, i);
+  }
+}
+
+template <int FMT, class T>
+__global__ __launch_bounds__(kThreads) void k_mx_dequantize(const uint8_t *__restrict__ elems,
+                                                            const uint8_t *__restrict__ scales, T *__restrict__ out,
+                                                            size_t n8) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < n8; i += (size_t)gridDim.x * kThreads) {
+    const float s = mx_scale(scales[i >> 2]);
+    float v[8];
+    if constexpr (FMT == kMxFp8) {
+      const uint2 q = reinterpret_cast<const uint2 *>(elems)[i];
+      const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, true);
+      const v2f c = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, true);
+      v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
+    } else {
+      const uint32_t q = reinterpret_cast<const uint32_t *>(elems)[i];
+      const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 1);
+      const v2f c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 3);
+      v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= s;
+    store8(out + 8 * i, v);
+  }
+}
+
+// Sum of one double per thread over a workgroup of whole waves; `red` is a
+// fresh array of 16 for each call.
+RT_DEV double block_sum_f64(double v, double *red) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double s = 0.0;
+  for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += red[i];
+  return s;
+}
+
+// y as the f32 next to it that is odd in its last place, unless y is an f32: a
+// second rounding to fewer bits then goes the way a single one would.
+RT_DEV float f32_odd(double y) {
+  const float f = (float)y;
+  const uint32_t b = f32_bits(f);
+  if ((double)f == y || (b & 1)) return f;
+  return bits_f32(__builtin_fabs(y) > __builtin_fabs((double)f) ? b + 1 : b - 1);
+}
+
+// One workgroup per row, the row in registers: G groups of eight per thread.
+//   u = x or x / rms(x) (1 + post);  h = residual + u;  y = h / rms(h) (1 + gamma)
+// The row's arithmetic is in 64 bits (about ten operations per element against
+// 13 bytes of memory: not what bounds it), so that y is rounded once, to its
+// element, and h once, to f32.
+template <int FMT, class T, int G>
+__global__ __launch_bounds__(1024) void k_add_rmsnorm_mx(const T *x, const float *residual,
+                                                         const float *__restrict__ post,
+                                                         const float *__restrict__ gamma, double eps,
+                                                         uint8_t *__restrict__ elems, uint8_t *__restrict__ scales,
+                                                         float *sum_out, int k, size_t row0) {
+  __shared__ double red[2][16];
+  const size_t row = row0 + blockIdx.x, base = row * (size_t)k;
+  const int groups = k >> 3;
+  double h[G][8];
+  double ss = 0.0;
+#pragma unroll
+  for (int j = 0; j < G; ++j) {
+    const int c = (int)threadIdx.x + j * (int)blockDim.x;
+    float v[8] = {};
+    if (c < groups) load8(x + base + 8 * c, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      h[j][i] = (double)v[i];
+      ss = __builtin_fma(h[j][i], h[j][i], ss);
+    }
+  }
+  if (post) {
+    const double r = 1.0 / __builtin_sqrt(block_sum_f64(ss, red[0]) / k + eps);
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int c = (int)threadIdx.x + j * (int)blockDim.x;
+      float g[8] = {};
+      if (c < groups) load8(post + 8 * c, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[j][i] *= r * (1.0 + (double)g[i]);
+    }
+  }
+  if (post || residual) {
+    ss = 0.0;
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int c = (int)threadIdx.x + j * (int)blockDim.x;
+      float v[8] = {};
+      if (residual && c < groups) load8(residual + base + 8 * c, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        h[j][i] += (double)v[i];
+        ss = __builtin_fma(h[j][i], h[j][i], ss);
+      }
+    }
+  }
+  const double r = 1.0 / __builtin_sqrt(block_sum_f64(ss, red[1]) / k + eps);
+#pragma unroll
+  for (int j = 0; j < G; ++j) {
+    const int c = (int)threadIdx.x + j * (int)blockDim.x;
+    if (c >= groups) continue;  // groups % 4 == 0: a quad is in or out as a whole
+    float v[8], g[8];
+    if (sum_out) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (float)h[j][i];
+      store8(sum_out + base + 8 * c, v);
+    }
+    load8(gamma + 8 * c, g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = f32_odd(h[j][i] * r * (1.0 + (double)g[i]));
+    mx_store8<FMT>(v, elems, scales, base / 8 + c);
+  }
+}
+
+// gelu_tanh(v) = v / (1 + e^(-2y)), y = sqrt(2/pi) (v + 0.044715 v^3): the same
+// function as the decode step's activation, in the form that keeps its relative
+// accuracy where it goes to zero (a block of 32 small outputs has its own scale).
+RT_DEV float gelu_rel(float v) {
+  constexpr float c = -2.0f * 0.7978845608028654f * 1.4426950408889634f;
+  const float z = v * __builtin_fmaf(c * 0.044715f, v * v, c);  // -2y log2(e)
+  const float d = 1.0f + __builtin_amdgcn_exp2f(fminf(z, 126.f));
+  const float r = __builtin_amdgcn_rcpf(d);
+  // past 2^126 the quotient is below every normal number: zero, as the infinite power would give
+  return v * (z > 126.f ? 0.f : __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r));
+}
+
+template <int FMT, class T>
+__global__ __launch_bounds__(kThreads) void k_gelu_mul_mx(const T *__restrict__ gate, const T *__restrict__ up,
+                                                          size_t ld, uint8_t *__restrict__ elems,
+                                                          uint8_t *__restrict__ scales, size_t n8, uint32_t groups) {
+  for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < n8; i += (size_t)gridDim.x * kThreads) {
+    const size_t row = n8 >> 32 ? i / groups : (size_t)((uint32_t)i / groups);
+    const size_t at = row * ld + 8 * (i - row * groups);
+    float g[8], u[8];
+    load8(gate + at, g);
+    load8(up + at, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = gelu_rel(g[j]) * u[j];
+    mx_store8<FMT>(g, elems, scales, i);
+  }
+}
+
+dim3 grid_for(size_t n8) {
+  const size_t g = (n8 + kThreads - 1) / kThreads;
+  return dim3((unsigned)(g < (size_t)kMaxGrid ? g : (size_t)kMaxGrid));
+}
+
+template <int FMT, class T>
+void norm_launch(const T *x, const float *residual, const float *post, const float *gamma, float eps, uint8_t *elems,
+                 uint8_t *scales, float *sum_out, size_t rows, int k, hipStream_t s) {
+  const int groups = k / 8, per = (groups + 1023) / 1024;  // groups of eight per thread, at most 4 (k <= kNormMaxK)
+  const int g = per <= 1 ? 1 : per <= 2 ? 2 : 4;
+  const dim3 block(((groups + g - 1) / g + 63) / 64 * 64);
+  auto kern = g == 1 ? k_add_rmsnorm_mx<FMT, T, 1> : g == 2 ? k_add_rmsnorm_mx<FMT, T, 2> : k_add_rmsnorm_mx<FMT, T, 4>;
+  constexpr size_t kRowsPerLaunch = 1 << 21;  // a grid's threads stay below 2^32
+  for (size_t r0 = 0; r0 < rows; r0 += kRowsPerLaunch)
+    hipLaunchKernelGGL(kern, dim3((unsigned)std::min(rows - r0, kRowsPerLaunch)), block, 0, s, x, residual, post, gamma,
+                       (double)eps, elems, scales, sum_out, k, r0);
+}
+
+}  // namespace
+
+hipError_t launch_mx_quantize(int fmt, const void *x, bool bf16, void *out, size_t n, hipStream_t s) {
+  uint8_t *e = static_cast<uint8_t *>(out), *sc = e + mx_elem_bytes(fmt, n);
+  const dim3 g = grid_for(n / 8), b(kThreads);
+  const float *xf = static_cast<const float *>(x);
+  const uint16_t *xh = static_cast<const uint16_t *>(x);
+  if (fmt == kMxFp8) {
+    if (bf16) hipLaunchKernelGGL((k_mx_quantize<kMxFp8, uint16_t>), g, b, 0, s, xh, e, sc, n / 8);
+    else hipLaunchKernelGGL((k_mx_quantize<kMxFp8, float>), g, b, 0, s, xf, e, sc, n / 8);
+  } else {
+    if (bf16) hipLaunchKernelGGL((k_mx_quantize<kMxFp4, uint16_t>), g, b, 0, s, xh, e, sc, n / 8);
+    else hipLaunchKernelGGL((k_mx_quantize<kMxFp4, float>), g, b, 0, s, xf, e, sc, n / 8);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_mx_dequantize(int fmt, const void *src, void *out, bool bf16, size_t n, hipStream_t s) {
+  const uint8_t *e = static_cast<const uint8_t *>(src), *sc = e + mx_elem_bytes(fmt, n);
+  const dim3 g = grid_for(n / 8), b(kThreads);
+  float *of = static_cast<float *>(out);
+  uint16_t *oh = static_cast<uint16_t *>(out);
+  if (fmt == kMxFp8) {
+    if (bf16) hipLaunchKernelGGL((k_mx_dequantize<kMxFp8, uint16_t>), g, b, 0, s, e, sc, oh, n / 8);
+    else hipLaunchKernelGGL((k_mx_dequantize<kMxFp8, float>), g, b, 0, s, e, sc, of, n / 8);
+  } else {
+    if (bf16) hipLaunchKernelGGL((k_mx_dequantize<kMxFp4, uint16_t>), g, b, 0, s, e, sc, oh, n / 8);
+    else hipLaunchKernelGGL((k_mx_dequantize<kMxFp4, float>), g, b, 0, s, e, sc, of, n / 8);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_add_rmsnorm_mx(int fmt, const void *x, bool bf16, const float *residual, const float *post,
+                                 const float *gamma, float eps, void *out, float *sum_out, size_t rows, int k,
+                                 hipStream_t s) {
+  uint8_t *e = static_cast<uint8_t *>(out), *sc = e + mx_elem_bytes(fmt, rows * (size_t)k);
+  const float *xf = static_cast<const float *>(x);
+  const uint16_t *xh = static_cast<const uint16_t *>(x);
+  if (fmt == kMxFp8) {
+    if (bf16) norm_launch<kMxFp8>(xh, residual, post, gamma, eps, e, sc, sum_out, rows, k, s);
+    else norm_launch<kMxFp8>(xf, residual, post, gamma, eps, e, sc, sum_out, rows, k, s);
+  } else {
+    if (bf16) norm_launch<kMxFp4>(xh, residual, post, gamma, eps, e, sc, sum_out, rows, k, s);
+    else norm_launch<kMxFp4>(xf, residual, post, gamma, eps, e, sc, sum_out, rows, k, s);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_gelu_mul_mx(int fmt, const void *gate, const void *up, bool bf16, size_t ld, void *out, size_t rows,
+                              int k, hipStream_t s) {
+  const size_t n = rows * (size_t)k;
+  uint8_t *e = static_cast<uint8_t *>(out), *sc = e + mx_elem_bytes(fmt, n);
+  const dim3 g = grid_for(n / 8), b(kThreads);
+  const uint32_t groups = (uint32_t)k / 8;
+  const float *gf = static_cast<const float *>(gate), *uf = static_cast<const float *>(up);
+  const uint16_t *gh = static_cast<const uint16_t *>(gate), *uh = static_cast<const uint16_t *>(up);
+  if (fmt == kMxFp8) {
+    if (bf16) hipLaunchKernelGGL((k_gelu_mul_mx<kMxFp8, uint16_t>), g, b, 0, s, gh, uh, ld, e, sc, n / 8, groups);
+    else hipLaunchKernelGGL((k_gelu_mul_mx<kMxFp8, float>), g, b, 0, s, gf, uf, ld, e, sc, n / 8, groups);
+  } else {
+    if (bf16) hipLaunchKernelGGL((k_gelu_mul_mx<kMxFp4, uint16_t>), g, b, 0, s, gh, uh, ld, e, sc, n / 8, groups);
+    else hipLaunchKernelGGL((k_gelu_mul_mx<kMxFp4, float>), g, b, 0, s, gf, uf, ld, e, sc, n / 8, groups);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace rt

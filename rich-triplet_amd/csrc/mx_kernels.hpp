@@ -1,0 +1,29 @@
+// mx_kernels.hpp -- host-side launchers of the microscaled kernels.  Arguments
+// are validated by the C ABI layer (mx_capi.hip) before any of these is called.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace rt {
+
+// Elements of one RMSNorm row: held in the registers of one workgroup.
+constexpr int kNormMaxK = 1024 * 8 * 4;
+
+// n elements (whole blocks of 32), fmt kMxFp8 or kMxFp4; x / out f32 or bf16 bits.
+hipError_t launch_mx_quantize(int fmt, const void *x, bool bf16, void *out, size_t n, hipStream_t s);
+hipError_t launch_mx_dequantize(int fmt, const void *src, void *out, bool bf16, size_t n, hipStream_t s);
+hipError_t launch_add_rmsnorm_mx(int fmt, const void *x, bool bf16, const float *residual, const float *post,
+                                 const float *gamma, float eps, void *out, float *sum_out, size_t rows, int k,
+                                 hipStream_t s);
+hipError_t launch_gelu_mul_mx(int fmt, const void *gate, const void *up, bool bf16, size_t ld, void *out, size_t rows,
+                              int k, hipStream_t s);
+
+// c[m][n] = a[m][k] . W[n][k] (+ bias[n]), W MXFP4 planar, c f32 or bf16 bits.
+enum MxAct { kMxActF32, kMxActBf16, kMxActFp8, kMxActFp4 };
+size_t mx_gemm_workspace_bytes(MxAct act, int m, int n, int k);
+hipError_t launch_mx_gemm(MxAct act, const void *a, const void *w, const float *bias, void *c, bool c_bf16, int m,
+                          int n, int k, void *ws, hipStream_t s);
+
+}  // namespace rt
