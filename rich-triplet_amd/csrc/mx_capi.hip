@@ -30,6 +30,9 @@ rt_status check_product(const char *who, const void *a, const void *w, const flo
     return set_error(RT_EINVAL, "%s: m=%lld n=%lld k=%lld must be positive", who, (long long)m, (long long)n, (long long)k);
   if (k % kMxBlock != 0) return set_error(RT_EINVAL, "%s: k=%lld must be a multiple of 32", who, (long long)k);
   if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return set_error(RT_EINVAL, "%s: m, n or k exceeds int32", who);
+  // 256 rows of either operand stay below 2^31 bytes, the tiles of c below 2^31
+  if (k > (1 << 22) || m > (int64_t(1) << 40) / n)
+    return set_error(RT_EINVAL, "%s: m=%lld n=%lld k=%lld is too large", who, (long long)m, (long long)n, (long long)k);
   if (!a || !w || !c) return set_error(RT_EINVAL, "%s: null pointer", who);
   if (!aligned16(a) || !aligned16(w)) return set_error(RT_EINVAL, "%s: a and w must be 16-byte aligned", who);
   if ((reinterpret_cast<uintptr_t>(c) & (c_bf16 ? 1u : 3u)) != 0)
@@ -42,12 +45,11 @@ rt_status check_product(const char *who, const void *a, const void *w, const flo
 
 rt_status rt::mx_product(const char *who, int act, const void *a, const void *w, const float *bias, void *c,
                          bool c_bf16, int64_t m, int64_t n, int64_t k, hipStream_t s) {
-  const size_t need = mx_gemm_workspace_bytes((MxAct)act, (int)m, (int)n, (int)k);
+  rt_status st = check_product(who, a, w, bias, c, c_bf16, m, n, k);
+  if (st != RT_OK) return st;
   void *ws = nullptr;
-  if (need) {
-    rt_status st = gemm_workspace(need, s, &ws);
-    if (st != RT_OK) return st;
-  }
+  st = gemm_workspace(mx_gemm_workspace_bytes((MxAct)act, (int)m, (int)n, (int)k), s, &ws);
+  if (st != RT_OK) return st;
   return hip_error(launch_mx_gemm((MxAct)act, a, w, bias, c, c_bf16, (int)m, (int)n, (int)k, ws, s), who);
 }
 
@@ -115,23 +117,17 @@ rt_status rt_mx_gemm(int32_t a_fmt, const void *a, const void *w, const float *b
   if (a_fmt != RT_MX_FP4 && a_fmt != RT_MX_FP8) return set_error(RT_EINVAL, "%s: format %d is neither RT_MX_FP4 nor RT_MX_FP8", who, a_fmt);
   if (c_type != RT_TYPE_F32 && c_type != RT_TYPE_BF16) return set_error(RT_EINVAL, "%s: type %d is neither RT_TYPE_F32 nor RT_TYPE_BF16", who, c_type);
   const bool bf16 = c_type == RT_TYPE_BF16;
-  rt_status st = check_product(who, a, w, bias, c, bf16, m, n, k);
-  if (st != RT_OK) return st;
   return mx_product(who, a_fmt == RT_MX_FP8 ? kMxActFp8 : kMxActFp4, a, w, bias, c, bf16, m, n, k, (hipStream_t)stream);
 }
 
 rt_status rt_mxfp4_gemm(int32_t a_type, const void *a, const void *w, float *c, int64_t m, int64_t n, int64_t k, void *stream) {
   static const char *who = "rt_mxfp4_gemm";
   if (a_type != RT_TYPE_F32 && a_type != RT_TYPE_BF16) return set_error(RT_EINVAL, "%s: type %d is neither RT_TYPE_F32 nor RT_TYPE_BF16", who, a_type);
-  rt_status st = check_product(who, a, w, nullptr, c, false, m, n, k);
-  if (st != RT_OK) return st;
   return mx_product(who, a_type == RT_TYPE_F32 ? kMxActF32 : kMxActBf16, a, w, nullptr, c, false, m, n, k, (hipStream_t)stream);
 }
 
 rt_status rt_mxfp4_gemv(const void *w, const float *x, float *y, int64_t n, int64_t k, void *stream) {
   static const char *who = "rt_mxfp4_gemv";
-  rt_status st = check_product(who, x, w, nullptr, y, false, 1, n, k);
-  if (st != RT_OK) return st;
   return mx_product(who, kMxActF32, x, w, nullptr, y, false, 1, n, k, (hipStream_t)stream);
 }
 

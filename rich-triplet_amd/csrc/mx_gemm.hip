@@ -29,8 +29,11 @@
 // product is the sum of the planes' products; W is never widened.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "mx_common.hpp"
 #include "mx_kernels.hpp"
+#include "mfma_common.hpp"
 #include "rt_device.hpp"
 
 namespace rt {
@@ -42,57 +45,93 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int kPlanesF32 = 5, kPlanesBf16 = 3, kPlaneShift = 5;
 
+// Scales in the order the tile kernel reads them: for each 128 rows and 128 of K
+// (a stage) [64 lanes][8 tiles of 16 rows], lane l holding row l % 16 of each
+// tile and block l / 16 of the stage, so that one 4- or 8-byte LDS read gives a
+// lane its scales of four or eight tiles and the instruction picks the byte.
+__host__ __device__ inline size_t packed_at(size_t row, int kb, int nk) {
+  return (((row >> 7) * nk + (kb >> 2)) * 64 + (kb & 3) * 16 + (row & 15)) * 8 + ((row >> 4) & 7);
+}
+size_t packed_bytes(size_t rows, int nk) { return (rows + 127) / 128 * nk * 512; }
+
 // Digit planes of activations [rows][k]: plane p at planes + p rows k, e4m3,
 // one scale byte per block (that of plane 0; plane p's is 5p less, so it is at
-// least 20).  A thread holds eight elements, a block is a quad.
+// least 20), packed.  A thread holds eight elements, a block is a quad.
 template <class T, int P>
-__global__ __launch_bounds__(256) void k_mx_split(const T *__restrict__ x, uint8_t *__restrict__ planes,
-                                                  uint8_t *__restrict__ scales, size_t n8) {
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n8; i += (size_t)gridDim.x * 256) {
-    float v[8];
-    load8(x + 8 * i, v);
-    // plane 0 is below 256: the exponent of the block's largest value less 7
-    const int e = (int)(quad_max_u32(absmax8_bits(v)) >> 23);
-    const bool bad = e == 255;
-    const int b = bad ? 255 : max(e - 7, kPlaneShift * (kPlanesF32 - 1));
-    float inv = bad ? 0.f : bits_f32((uint32_t)(254 - b) << 23);
+RT_DEV void split_group(const T *__restrict__ x, uint8_t *__restrict__ planes, uint8_t *__restrict__ scales, size_t i,
+                        size_t n8, uint32_t groups, int nk) {
+  float v[8];
+  load8(x + 8 * i, v);
+  // plane 0 is below 256: the exponent of the block's largest value less 7
+  const int e = (int)(quad_max_u32(absmax8_bits(v)) >> 23);
+  const bool bad = e == 255;
+  const int b = bad ? 255 : max(e - 7, kPlaneShift * (kPlanesF32 - 1));
+  float inv = bad ? 0.f : bits_f32((uint32_t)(254 - b) << 23);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = bad ? 0.f : v[j] * inv;
+  for (int j = 0; j < 8; ++j) v[j] = bad ? 0.f : v[j] * inv;
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      float t[8];
-      constexpr float kQuarters = 3145728.f;  // 1.5 2^21: a sum with it is rounded to 2^-2
+  for (int p = 0; p < P; ++p) {
+    float t[8];
+    constexpr float kQuarters = 3145728.f;  // 1.5 2^21: a sum with it is rounded to 2^-2
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = (v[j] + kQuarters) - kQuarters;
-      const uint2 q = fp8x8(t);
-      reinterpret_cast<uint2 *>(planes + (size_t)p * 8 * n8)[i] = q;
-      if (p + 1 < P) {
-        typedef float v2f __attribute__((ext_vector_type(2)));
-        const v2f d0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, false), d1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, true);
-        const v2f d2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, false), d3 = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, true);
-        const float d[8] = {d0.x, d0.y, d1.x, d1.y, d2.x, d2.y, d3.x, d3.y};
+    for (int j = 0; j < 8; ++j) t[j] = (v[j] + kQuarters) - kQuarters;
+    const uint2 q = fp8x8(t);
+    reinterpret_cast<uint2 *>(planes + (size_t)p * 8 * n8)[i] = q;
+    if (p + 1 < P) {
+      typedef float v2f __attribute__((ext_vector_type(2)));
+      const v2f d0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, false), d1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, true);
+      const v2f d2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, false), d3 = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, true);
+      const float d[8] = {d0.x, d0.y, d1.x, d1.y, d2.x, d2.y, d3.x, d3.y};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = (v[j] - d[j]) * 32.f;
-      }
+      for (int j = 0; j < 8; ++j) v[j] = (v[j] - d[j]) * 32.f;
     }
-    if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)b;
+  }
+  if ((threadIdx.x & 3) == 0) {
+    const size_t row = i / groups;
+    const int kb = (int)(i - row * groups) >> 2;
+    scales[packed_at(row, kb, nk)] = (uint8_t)b;
+    if (kb + 1 == (int)(groups >> 2))
+      for (int t = kb + 1; t < 4 * nk; ++t) scales[packed_at(row, t, nk)] = 127;  // zero elements lie there
   }
 }
 
-struct MxOperand {
-  const uint8_t *e, *s;
-  size_t plane;  // bytes from one digit plane to the next
-  int planes;
-};
-
-// Four e8m0 bytes of blocks 4t .. 4t+3 of a row of kb blocks (past its end 127:
-// the elements there are zero).
-RT_DEV int scale4(const uint8_t *row, int kb, int t) {
-  if ((kb & 3) == 0) return *reinterpret_cast<const int *>(row + 4 * t);
-  uint32_t v = 0;
+// Packs eight scales (one lane's of a stage) of a planar tensor's [rows][kb].
+RT_DEV void pack_group(const uint8_t *__restrict__ s, uint8_t *__restrict__ packed, size_t i, size_t rows, int kb, int nk) {
+  const int lane = (int)(i & 63), b = 4 * (int)((i >> 6) % nk) + (lane >> 4);
+  const size_t row0 = (i >> 6) / nk * 128 + (lane & 15);
+  uint32_t v[2] = {0x7F7F7F7Fu, 0x7F7F7F7Fu};
+  if (b < kb) {
+    v[0] = v[1] = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v |= (4 * t + i < kb ? (uint32_t)row[4 * t + i] : 127u) << (8 * i);
-  return (int)v;
+    for (int t = 0; t < 8; ++t) {
+      const size_t row = row0 + 16 * t;
+      v[t >> 2] |= (uint32_t)s[(row < rows ? row : rows - 1) * kb + b] << (8 * (t & 3));
+    }
+  }
+  reinterpret_cast<uint2 *>(packed)[i] = make_uint2(v[0], v[1]);
+}
+
+// What the tile kernel needs besides the operands' elements, in one launch:
+// workgroups below `wg_a` split the activations or pack their scales, the rest
+// pack the weight's.
+template <class T, int P>  // P = 0: microscaled activations, x their scales
+__global__ __launch_bounds__(256) void k_mx_prep(const T *__restrict__ x, uint8_t *__restrict__ planes,
+                                                 uint8_t *__restrict__ as, const uint8_t *__restrict__ wscale,
+                                                 uint8_t *__restrict__ ws, size_t M, size_t N, int K, int nk,
+                                                 unsigned wg_a) {
+  const bool on_a = blockIdx.x < wg_a;
+  const size_t first = (size_t)(on_a ? blockIdx.x : blockIdx.x - wg_a) * 256 + threadIdx.x;
+  const size_t step = (size_t)(on_a ? wg_a : gridDim.x - wg_a) * 256;
+  if (!on_a) {
+    const size_t n = (N + 127) / 128 * nk * 64;
+    for (size_t i = first; i < n; i += step) pack_group(wscale, ws, i, N, K / 32, nk);
+  } else if constexpr (P == 0) {
+    const size_t n = (M + 127) / 128 * nk * 64;
+    for (size_t i = first; i < n; i += step) pack_group(x, as, i, M, K / 32, nk);
+  } else {
+    const size_t n8 = M * (size_t)K / 8;
+    for (size_t i = first; i < n8; i += step) split_group<T, P>(x, planes, as, i, n8, (uint32_t)K / 8, nk);
+  }
 }
 
 // The elements of 2 and above of four e4m3 bytes (bit 6 is the exponent field's
@@ -102,97 +141,345 @@ RT_DEV uint32_t fp8_upper(uint32_t x) {
   return x & ((t << 8) - t);
 }
 
-// One wave per 16 x 16 of c, operands straight from memory.
-template <int FA, bool TWO, class C>
-__global__ __launch_bounds__(256) void k_mx_gemm_direct(MxOperand a, MxOperand w, const float *__restrict__ bias,
-                                                        C *__restrict__ c, int M, int N, int K) {
-  const int lane = (int)threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int n0 = ((int)blockIdx.x * 4 + ((int)threadIdx.x >> 6)) * 16, m0 = (int)blockIdx.y * 16;
-  const int kb = K / 32, nr = min(n0 + l16, N - 1), mr = min(m0 + l16, M - 1);
-  const uint8_t *we = w.e + (size_t)nr * (K / 2), *ws = w.s + (size_t)nr * kb;
-  const uint8_t *as = a.s + (size_t)mr * kb;
-  v4f acc = {0.f, 0.f, 0.f, 0.f};
-  for (int t = 0; t < (kb + 3) / 4; ++t) {
-    const v4i zero = {0, 0, 0, 0};
-    const int b = 4 * t + g;
-    const v4i wq = b < kb ? *reinterpret_cast<const v4i *>(we + (size_t)b * 16) : zero;
-    const v8i wv = {wq[0], wq[1], wq[2], wq[3], 0, 0, 0, 0};
-    const int wsc = (int)((uint32_t)scale4(ws, kb, t) >> (8 * g)), asc = scale4(as, kb, t) >> (8 * g);
-    for (int p = 0; p < a.planes; ++p) {
-      v8i av;
-      if constexpr (FA == kMxFp8) {
-        // a lane's 32 bytes are two half blocks, 64 of K apart
-        const uint8_t *ae = a.e + (size_t)p * a.plane + (size_t)mr * K;
-        const int b0 = 4 * t + (g >> 1), b1 = b0 + 2;
-        const v4i x = b0 < kb ? *reinterpret_cast<const v4i *>(ae + (size_t)b0 * 32 + 16 * (g & 1)) : zero;
-        const v4i y = b1 < kb ? *reinterpret_cast<const v4i *>(ae + (size_t)b1 * 32 + 16 * (g & 1)) : zero;
-        av = (v8i){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      } else {
-        const v4i x = b < kb ? *reinterpret_cast<const v4i *>(a.e + (size_t)mr * (K / 2) + (size_t)b * 16) : zero;
-        av = (v8i){x[0], x[1], x[2], x[3], 0, 0, 0, 0};
-      }
-      const int ab = (asc & 255) == 255 ? 255 : (asc & 255) - kPlaneShift * p;
-      if constexpr (TWO) {
-        v8i up;
+RT_DEV uint32_t lds_addr(const void *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p; }
+// LDS reads at an address plus a constant, waited for by lds_wait_n (see lds_read16).
+template <int OFF>
+RT_DEV u32x4 lds_b128(uint32_t a) {
+  static_assert(OFF >= 0 && OFF < 65536, "16-bit offset");
+  u32x4 v;
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(a), "n"(OFF));
+  return v;
+}
+RT_DEV uint32_t lds_b32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ds_read_b32 %0, %1" : "=v"(v) : "v"(a));
+  return v;
+}
+// Waits until at most N LDS operations are outstanding; the operands' readers come after it.
+template <int N>
+RT_DEV void lds_wait_n(u32x4 &v) {
+  asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(v) : "n"(N));
+}
+template <int N>
+RT_DEV void lds_wait_n(uint32_t &v) {
+  asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(v) : "n"(N));
+}
+
+template <int V>
+struct IntC {
+  static constexpr int value = V;
+};
+template <int N, class F, int I = 0>
+RT_DEV void steps(F f) {  // f(IntC<0>), ..., f(IntC<N-1>)
+  if constexpr (I < N) {
+    f(IntC<I>{});
+    steps<N, F, I + 1>(f);
+  }
+}
+
+// Copies 16 bytes per lane from base + voff + soff to `to` + 16 lane; a lane whose
+// voff is negative reads out of the buffer's range, which leaves zeros in LDS.
+// (A function: the host pass has no buffer descriptors.)
+RT_DEV void copy_to_lds(const uint8_t *base, uint8_t *to, int voff, int soff) {
+  const auto buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, 0x7FFFFFFF, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lvoid *)to, 16, voff, soff, 0, 0);
+}
+
+struct TileArgs {
+  const uint8_t *a, *w;    // elements: a [planes][M][K], w [N][K]
+  const uint8_t *as, *ws;  // packed scales
+  size_t plane;            // bytes of one digit plane
+  const float *bias;
+  void *c;      // the result, or (ksplit > 1) the f32 partials [ksplit][M][N]
+  int M, N, K, nk, planes, tiles_m, tiles_n, ksplit;
+  bool vec;  // 16-byte (bf16: 8-byte) stores of four columns
+};
+
+// C tile of 16 NT WN columns (n) by 16 MT WM rows (m) by WN x WM waves, K in
+// stages of 128 through three LDS slots: while a stage is multiplied the copies
+// of the next two are on their way, one barrier per stage.
+//
+// A slot row is a row's 64 (e2m1) or 128 (e4m3) bytes of the stage, in 16-byte
+// units; unit u of row r lies at u ^ (r / 4 % 4) or u ^ (r / 2 % 8), so that the 16
+// rows of a fragment read hit 16 different bank groups.  Past the end of K the
+// copies read out of their buffer's range, which leaves zeros in LDS.
+template <int FA, bool TWO, int WN, int WM, int NT, int MT, class C>
+__global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
+  constexpr int kWaves = WN * WM, BN = 16 * NT * WN, BM = 16 * MT * WM;
+  constexpr int kARow = FA == kMxFp8 ? 128 : 64, kWBytes = BN * 64, kABytes = BM * kARow;
+  constexpr int kWScale = kWBytes + kABytes, kAScale = kWScale + BN * 4, kSlot = kAScale + BM * 4;
+  constexpr int kWCopies = kWBytes / 1024 / kWaves, kACopies = kABytes / 1024 / kWaves;
+  static_assert(kWBytes % (1024 * kWaves) == 0 && kABytes % (1024 * kWaves) == 0, "whole copies per wave");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[3 * kSlot];
+  const int tid = (int)threadIdx.x, lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
+  // XCD b % 8 gets a contiguous run of tiles, walked in groups of eight tile rows
+  const int ntiles = g.tiles_m * g.tiles_n, x8 = (int)blockIdx.x & 7, r8 = ntiles & 7, q8 = ntiles >> 3;
+  const int tile = (x8 < r8 ? x8 * (q8 + 1) : r8 * (q8 + 1) + (x8 - r8) * q8) + ((int)blockIdx.x >> 3);
+  const int group = tile / (8 * g.tiles_n), in_group = tile % (8 * g.tiles_n), gm = min(8, g.tiles_m - group * 8);
+  const int tm = group * 8 + in_group % gm, tn = in_group / gm;
+  const int m0 = tm * BM, n0 = tn * BN, kb = g.K / 32;
+  const int total = g.planes * g.nk, split = (int)blockIdx.y;
+  const int u0 = (int)((int64_t)split * total / g.ksplit), u1 = (int)((int64_t)(split + 1) * total / g.ksplit);
+
+  // Copies: this lane's byte offsets from the tile's first row, and its unit's
+  // block within a stage (to tell where the row ends).
+  const size_t wrow = (size_t)g.K / 2, arow = FA == kMxFp8 ? (size_t)g.K : wrow;
+  uint32_t wo[kWCopies], ao[kACopies];
+  const int wslot = lane & 3;
+  int wblk[kWCopies], ablk[kACopies];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) up[i] = (int)fp8_upper((uint32_t)av[i]), av[i] ^= up[i];
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, up, acc, 4, 0, 0, wsc, 0, ab);
-      }
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, av, acc, 4, FA == kMxFp8 ? 0 : 4, 0, wsc, 0, ab);
+  for (int i = 0; i < kWCopies; ++i) {
+    const int r = 16 * (kWCopies * wave + i) + (lane >> 2), u = wslot ^ ((r >> 2) & 3);
+    wo[i] = (uint32_t)(min(n0 + r, g.N - 1) - n0) * (uint32_t)wrow + 16 * u;
+    wblk[i] = u;
+  }
+#pragma unroll
+  for (int i = 0; i < kACopies; ++i) {
+    if constexpr (FA == kMxFp8) {
+      const int r = 8 * (kACopies * wave + i) + (lane >> 3), u = (lane & 7) ^ ((r >> 1) & 7);
+      ao[i] = (uint32_t)(min(m0 + r, g.M - 1) - m0) * (uint32_t)arow + 16 * u;
+      ablk[i] = u >> 1;
+    } else {
+      const int r = 16 * (kACopies * wave + i) + (lane >> 2), u = (lane & 3) ^ ((r >> 2) & 3);
+      ao[i] = (uint32_t)(min(m0 + r, g.M - 1) - m0) * (uint32_t)arow + 16 * u;
+      ablk[i] = u;
     }
   }
-  const int row = m0 + l16;
-  if (row >= M) return;
+  const uint8_t *wb = g.w + (size_t)n0 * wrow;
+  // scales: 512 bytes per 128 rows and stage; the copying lanes' pieces
+  const int sl = lane & 31, sh = lane >> 5;
+  auto scale_src = [&](const uint8_t *s, int row0, int rows, int tile_rows, int j) __attribute__((always_inline)) {
+    const int last = (rows - 1) >> 7;  // a 256-row tile's second half may lie past the end: read the last again
+    const int blk = min((row0 >> 7) + (tile_rows == 256 ? sh : 0), last);
+    return s + ((size_t)blk * g.nk + j) * 512 + 16 * sl;
+  };
+  auto issue = [&](int u, int slot) __attribute__((always_inline)) {
+    const int p = g.planes == 1 ? 0 : u / g.nk, j = u - p * g.nk;
+    uint8_t *base = lds + slot * kSlot;
+    if (wave == 0 && (BN == 256 || lane < 32))
+      __builtin_amdgcn_global_load_lds((gvoid *)scale_src(g.ws, n0, g.N, BN, j), (lvoid *)(base + kWScale), 16, 0, 0);
+    if (wave == 1 && (BM == 256 || lane < 32))
+      __builtin_amdgcn_global_load_lds((gvoid *)scale_src(g.as, m0, g.M, BM, j), (lvoid *)(base + kAScale), 16, 0, 0);
+    const uint8_t *ab = g.a + (size_t)p * g.plane + (size_t)m0 * arow;
+    const int left = kb - 4 * j;  // blocks of the row from this stage on
+    constexpr int kOut = (int)0x80000000;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int n = n0 + 4 * g + r;
-    if (n >= N) continue;
-    const float v = acc[r] + (bias ? bias[n] : 0.f);
-    if constexpr (sizeof(C) == 4) c[(size_t)row * N + n] = v;
-    else c[(size_t)row * N + n] = f32_to_bf16_bits(v);
+    for (int i = 0; i < kWCopies; ++i)
+      copy_to_lds(wb, base + (kWCopies * wave + i) * 1024, wblk[i] < left ? (int)wo[i] : kOut, j * 64);
+#pragma unroll
+    for (int i = 0; i < kACopies; ++i)
+      copy_to_lds(ab, base + kWBytes + (kACopies * wave + i) * 1024, ablk[i] < left ? (int)ao[i] : kOut, j * kARow);
+  };
+
+  // Fragments: row l16 of tile i is 16 rows further per tile, whole swizzle periods.
+  const uint32_t lb = lds_addr(lds);
+  const uint32_t fw = lb + (16 * NT * wn + l16) * 64 + 16 * (grp ^ ((l16 >> 2) & 3));
+  const uint32_t fa0 = lb + kWBytes + (16 * MT * wm + l16) * kARow +
+                       16 * (FA == kMxFp8 ? grp ^ ((l16 >> 1) & 7) : grp ^ ((l16 >> 2) & 3));
+  const uint32_t fa1 = lb + kWBytes + (16 * MT * wm + l16) * kARow + 16 * ((4 + grp) ^ ((l16 >> 1) & 7));
+  // a lane's scale bytes: [128 rows][64 lanes][8 tiles]
+  const uint32_t fws = lb + kWScale + (NT * wn / 8) * 512 + lane * 8 + (NT * wn) % 8;
+  const uint32_t fas = lb + kAScale + (MT * wm / 8) * 512 + lane * 8 + (MT * wm) % 8;
+
+  v4f acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+
+  if (u0 < u1) issue(u0, 0);
+  if (u0 + 1 < u1) issue(u0 + 1, 1);
+  int slot = 0;
+  for (int u = u0; u < u1; ++u) {
+    // this wave's copies of stage u (those of u+1 may be on their way), then everyone's
+    if (u + 1 < u1) wait_vmcnt<kWCopies + kACopies>();
+    else wait_vmcnt<0>();
+    wg_barrier();
+    // the slot of stage u+2 was read in stage u-1, by every wave before this barrier
+    if (u + 2 < u1) issue(u + 2, slot == 0 ? 2 : slot - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t so = (uint32_t)slot * kSlot;
+    uint32_t sw[NT / 4], sa[MT / 4];
+    u32x4 wf[NT], af[MT][FA == kMxFp8 ? 2 : 1];
+#pragma unroll
+    for (int i = 0; i < NT / 4; ++i) sw[i] = lds_b32(fws + so + 4 * i);
+#pragma unroll
+    for (int i = 0; i < MT / 4; ++i) sa[i] = lds_b32(fas + so + 4 * i);
+    steps<NT>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value;
+      wf[i] = lds_b128<i * 1024>(fw + so);
+    });
+    steps<MT>([&](auto jc) __attribute__((always_inline)) {
+      constexpr int j = decltype(jc)::value;
+      af[j][0] = lds_b128<j * 16 * kARow>(fa0 + so);
+      if constexpr (FA == kMxFp8) af[j][1] = lds_b128<j * 16 * kARow>(fa1 + so);
+    });
+    constexpr int kPerM = FA == kMxFp8 ? 2 : 1;
+    lds_wait_n<MT * kPerM>(sw[0]);
+#pragma unroll
+    for (int i = 0; i < NT / 4; ++i) lds_wait_n<MT * kPerM>(sw[i]);
+#pragma unroll
+    for (int i = 0; i < MT / 4; ++i) lds_wait_n<MT * kPerM>(sa[i]);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) lds_wait_n<MT * kPerM>(wf[i]);
+    if (g.planes > 1) {
+      const uint32_t less = 0x01010101u * kPlaneShift * (uint32_t)(u / g.nk);
+#pragma unroll
+      for (int i = 0; i < MT / 4; ++i) sa[i] -= less;  // no borrow: a digit block's byte is at least 20
+    }
+    steps<MT>([&](auto jc) __attribute__((always_inline)) {
+      constexpr int j = decltype(jc)::value, kLeft = (MT - 1 - j) * kPerM;
+#pragma unroll
+      for (int t = 0; t < kPerM; ++t) lds_wait_n<kLeft>(af[j][t]);
+      v8i av = {(int)af[j][0][0], (int)af[j][0][1], (int)af[j][0][2], (int)af[j][0][3], 0, 0, 0, 0};
+      if constexpr (FA == kMxFp8)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) av[4 + t] = (int)af[j][1][t];
+      v8i up = av;
+      if constexpr (TWO) {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) up[t] = (int)fp8_upper((uint32_t)av[t]), av[t] ^= up[t];
+      }
+      steps<NT>([&](auto ic) __attribute__((always_inline)) {
+        constexpr int i = decltype(ic)::value;
+        const v8i wv = {(int)wf[i][0], (int)wf[i][1], (int)wf[i][2], (int)wf[i][3], 0, 0, 0, 0};
+        if constexpr (TWO)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, up, acc[i][j], 4, 0, i & 3, (int)sw[i / 4],
+                                                                       j & 3, (int)sa[j / 4]);
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, av, acc[i][j], 4, FA == kMxFp8 ? 0 : 4, i & 3,
+                                                                     (int)sw[i / 4], j & 3, (int)sa[j / 4]);
+      });
+    });
+    slot = slot == 2 ? 0 : slot + 1;
+  }
+
+  // Lane: columns 4 grp .. + 3 of each 16, row l16.
+  const bool part = g.ksplit > 1;
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    const int row = m0 + 16 * (MT * wm + j) + l16;
+    if (row >= g.M) continue;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int col = n0 + 16 * (NT * wn + i) + 4 * grp;
+      if (col >= g.N) continue;
+      v4f v = acc[i][j];
+      if (part) {
+        float *d = static_cast<float *>(g.c) + ((size_t)split * g.M + row) * g.N + col;
+        if (g.vec) *reinterpret_cast<v4f *>(d) = v;
+        else
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (col + t < g.N) d[t] = v[t];
+        continue;
+      }
+      if (g.bias)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[t] += g.bias[min(col + t, g.N - 1)];
+      C *d = static_cast<C *>(g.c) + (size_t)row * g.N + col;
+      if constexpr (sizeof(C) == 4) {
+        if (g.vec) *reinterpret_cast<v4f *>(d) = v;
+        else
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (col + t < g.N) d[t] = v[t];
+      } else {
+        if (g.vec) *reinterpret_cast<uint2 *>(d) = make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
+        else
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (col + t < g.N) d[t] = f32_to_bf16_bits(v[t]);
+      }
+    }
+  }
+}
+
+// c[m][n] = sum over the K splits, in their order, + bias.
+template <class C>
+__global__ __launch_bounds__(256) void k_mx_sum(const float *__restrict__ part, const float *__restrict__ bias,
+                                                C *__restrict__ c, size_t mn, int N, int ks) {
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < mn; i += (size_t)gridDim.x * 256) {
+    float v = part[i];
+    for (int s = 1; s < ks; ++s) v += part[(size_t)s * mn + i];
+    if (bias) v += bias[i % N];
+    if constexpr (sizeof(C) == 4) c[i] = v;
+    else c[i] = f32_to_bf16_bits(v);
   }
 }
 
 size_t r256(size_t b) { return (b + 255) & ~size_t(255); }
 int planes_of(MxAct act) { return act == kMxActF32 ? kPlanesF32 : act == kMxActBf16 ? kPlanesBf16 : 1; }
+bool digits(MxAct act) { return act == kMxActF32 || act == kMxActBf16; }
+
+struct Plan {
+  int tile, ksplit;  // rows and columns of a C tile
+};
+Plan plan_for(MxAct act, int m, int n, int k) {
+  const int64_t t256 = (int64_t)((m + 255) / 256) * ((n + 255) / 256), t128 = (int64_t)((m + 127) / 128) * ((n + 127) / 128);
+  const int stages = planes_of(act) * ((k + 127) / 128);
+  if (t256 >= 256) return {256, 1};
+  int ks = (int)std::min<int64_t>(std::max<int64_t>(512 / t128, 1), 32);
+  ks = std::min(ks, std::max(stages / 4, 1));
+  return {128, ks};
+}
+
+template <int FA, bool TWO, class C>
+hipError_t tile_launch(const TileArgs &g, int tile, hipStream_t s) {
+  const dim3 grid(g.tiles_m * g.tiles_n, g.ksplit);
+  auto kern = tile == 256 ? k_mx_gemm_tile<FA, TWO, 2, 4, 8, 4, C> : k_mx_gemm_tile<FA, TWO, 2, 2, 4, 4, C>;
+  hipLaunchKernelGGL(kern, grid, dim3(tile == 256 ? 512 : 256), 0, s, g);
+  return hipGetLastError();
+}
 
 }  // namespace
 
 size_t mx_gemm_workspace_bytes(MxAct act, int m, int n, int k) {
-  if (act == kMxActFp8 || act == kMxActFp4) return 256;
-  return r256((size_t)planes_of(act) * m * k) + r256((size_t)m * (k / 32));
+  const int nk = (k + 127) / 128;
+  const Plan p = plan_for(act, m, n, k);
+  return (digits(act) ? r256((size_t)planes_of(act) * m * k) : 0) + r256(packed_bytes(m, nk)) + r256(packed_bytes(n, nk)) +
+         (p.ksplit > 1 ? (size_t)p.ksplit * m * n * 4 : 0);
 }
 
 hipError_t launch_mx_gemm(MxAct act, const void *a, const void *w, const float *bias, void *c, bool c_bf16, int m,
                           int n, int k, void *ws, hipStream_t s) {
-  const uint8_t *we = static_cast<const uint8_t *>(w);
-  const MxOperand W{we, we + (size_t)n * k / 2, 0, 1};
-  MxOperand A;
+  const int nk = (k + 127) / 128;
+  const Plan plan = plan_for(act, m, n, k);
   const size_t mk = (size_t)m * k;
-  if (act == kMxActF32 || act == kMxActBf16) {
-    uint8_t *pl = static_cast<uint8_t *>(ws), *sc = pl + r256(planes_of(act) * mk);
-    const dim3 g((unsigned)((mk / 8 + 255) / 256 < 65536 ? (mk / 8 + 255) / 256 : 65536)), b(256);
-    if (act == kMxActF32)
-      hipLaunchKernelGGL((k_mx_split<float, kPlanesF32>), g, b, 0, s, static_cast<const float *>(a), pl, sc, mk / 8);
-    else
-      hipLaunchKernelGGL((k_mx_split<uint16_t, kPlanesBf16>), g, b, 0, s, static_cast<const uint16_t *>(a), pl, sc, mk / 8);
-    A = {pl, sc, mk, planes_of(act)};
-  } else {
-    const uint8_t *ae = static_cast<const uint8_t *>(a);
-    A = {ae, ae + mx_elem_bytes(act == kMxActFp8 ? kMxFp8 : kMxFp4, mk), 0, 1};
-  }
-  const dim3 grid((n + 63) / 64, (m + 15) / 16), block(256);
-  float *cf = static_cast<float *>(c);
-  uint16_t *ch = static_cast<uint16_t *>(c);
-  if (act == kMxActFp4) {
-    if (c_bf16) hipLaunchKernelGGL((k_mx_gemm_direct<kMxFp4, false, uint16_t>), grid, block, 0, s, A, W, bias, ch, m, n, k);
-    else hipLaunchKernelGGL((k_mx_gemm_direct<kMxFp4, false, float>), grid, block, 0, s, A, W, bias, cf, m, n, k);
-  } else if (act == kMxActFp8) {
-    if (c_bf16) hipLaunchKernelGGL((k_mx_gemm_direct<kMxFp8, false, uint16_t>), grid, block, 0, s, A, W, bias, ch, m, n, k);
-    else hipLaunchKernelGGL((k_mx_gemm_direct<kMxFp8, true, float>), grid, block, 0, s, A, W, bias, cf, m, n, k);
-  } else {
-    hipLaunchKernelGGL((k_mx_gemm_direct<kMxFp8, false, float>), grid, block, 0, s, A, W, bias, cf, m, n, k);
-  }
+  uint8_t *p = static_cast<uint8_t *>(ws);
+  uint8_t *planes = p;
+  if (digits(act)) p += r256(planes_of(act) * mk);
+  uint8_t *as = p, *wsc = as + r256(packed_bytes(m, nk));
+  float *part = reinterpret_cast<float *>(wsc + r256(packed_bytes(n, nk)));
+  const uint8_t *we = static_cast<const uint8_t *>(w), *wscale = we + (size_t)n * k / 2;
+  const uint8_t *ae = static_cast<const uint8_t *>(a);
+
+  const size_t na = digits(act) ? mk / 8 : packed_bytes(m, nk) / 8, nw = packed_bytes(n, nk) / 8;
+  const unsigned wg_a = (unsigned)std::min<size_t>((na + 255) / 256, 1 << 16), wg_w = (unsigned)std::min<size_t>((nw + 255) / 256, 1 << 16);
+  const dim3 grid(wg_a + wg_w), block(256);
+  if (act == kMxActF32)
+    hipLaunchKernelGGL((k_mx_prep<float, kPlanesF32>), grid, block, 0, s, static_cast<const float *>(a), planes, as, wscale, wsc, (size_t)m, (size_t)n, k, nk, wg_a);
+  else if (act == kMxActBf16)
+    hipLaunchKernelGGL((k_mx_prep<uint16_t, kPlanesBf16>), grid, block, 0, s, static_cast<const uint16_t *>(a), planes, as, wscale, wsc, (size_t)m, (size_t)n, k, nk, wg_a);
+  else
+    hipLaunchKernelGGL((k_mx_prep<uint8_t, 0>), grid, block, 0, s, ae + mx_elem_bytes(act == kMxActFp8 ? kMxFp8 : kMxFp4, mk), nullptr, as, wscale, wsc, (size_t)m, (size_t)n, k, nk, wg_a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+
+  const bool to_part = plan.ksplit > 1;
+  void *out = to_part ? static_cast<void *>(part) : c;
+  const bool out16 = !to_part && c_bf16;
+  const TileArgs g{digits(act) ? planes : ae, we, as, wsc, mk, to_part ? nullptr : bias, out, m, n, k, nk, planes_of(act),
+                   (m + plan.tile - 1) / plan.tile, (n + plan.tile - 1) / plan.tile, plan.ksplit,
+                   n % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (out16 ? 7 : 15)) == 0};
+  if (act == kMxActFp4) e = out16 ? tile_launch<kMxFp4, false, uint16_t>(g, plan.tile, s) : tile_launch<kMxFp4, false, float>(g, plan.tile, s);
+  else if (act == kMxActFp8 && !c_bf16) e = tile_launch<kMxFp8, true, float>(g, plan.tile, s);
+  else e = out16 ? tile_launch<kMxFp8, false, uint16_t>(g, plan.tile, s) : tile_launch<kMxFp8, false, float>(g, plan.tile, s);
+  if (e != hipSuccess || !to_part) return e;
+  const size_t mn = (size_t)m * n;
+  const dim3 sg((unsigned)std::min<size_t>((mn + 255) / 256, 1 << 16));
+  if (c_bf16) hipLaunchKernelGGL(k_mx_sum<uint16_t>, sg, block, 0, s, part, bias, static_cast<uint16_t *>(c), mn, n, plan.ksplit);
+  else hipLaunchKernelGGL(k_mx_sum<float>, sg, block, 0, s, part, bias, static_cast<float *>(c), mn, n, plan.ksplit);
   return hipGetLastError();
 }
 

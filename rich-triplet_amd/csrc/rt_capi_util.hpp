@@ -16,7 +16,7 @@ bool aligned16(const void *p);
 // least `bytes`; RT_ESTATE if it would have to grow while the stream is captured.
 rt_status gemm_workspace(size_t bytes, hipStream_t stream, void **out);
 
-// c = a . W^T (+ bias) on an MXFP4 weight, arguments checked by the caller; act is an MxAct.
+// c = a . W^T (+ bias) on an MXFP4 weight, arguments checked here; act is an MxAct.
 rt_status mx_product(const char *who, int act, const void *a, const void *w, const float *bias, void *c, bool c_bf16,
                      int64_t m, int64_t n, int64_t k, hipStream_t s);
 
