@@ -43,11 +43,12 @@ struct IntC {
   static constexpr int value = V;
 };
 
-// P digit planes of eight values (two dwords of e4m3 each); a block is an
-// aligned quad of lanes.  Returns the scale byte of plane 0 (plane p's is 5p less,
-// so it is at least 20); a block with an infinity or a NaN has byte 255 and zeros.
-template <int P>
-RT_DEV uint32_t digits8(float (&v)[8], uint2 (&q)[P]) {
+// P digit planes of eight values, each handed to emit(p, two dwords of e4m3); a
+// block is an aligned quad of lanes.  Returns the scale byte of plane 0 (plane
+// p's is 5p less, so it is at least 20); a block with an infinity or a NaN has
+// byte 255 and zeros.
+template <int P, class F>
+RT_DEV uint32_t digits8(float (&v)[8], F emit) {
   typedef float v2f __attribute__((ext_vector_type(2)));
   const int e = (int)(quad_max_u32(absmax8_bits(v)) >> 23);
   const bool bad = e == 255;
@@ -55,7 +56,7 @@ RT_DEV uint32_t digits8(float (&v)[8], uint2 (&q)[P]) {
   const float inv = bad ? 0.f : bits_f32((uint32_t)(254 - b) << 23);
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = bad ? 0.f : v[j] * inv;
-#pragma unroll
+#pragma unroll 1
   for (int p = 0; p < P; ++p) {
     constexpr float kQuarters = 3145728.f;  // 1.5 2^21: a sum with it is rounded to 2^-2
     float t[8];
@@ -65,17 +66,30 @@ RT_DEV uint32_t digits8(float (&v)[8], uint2 (&q)[P]) {
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(t[2], t[3], lo, true);
     int hi = __builtin_amdgcn_cvt_pk_fp8_f32(t[4], t[5], 0, false);
     hi = __builtin_amdgcn_cvt_pk_fp8_f32(t[6], t[7], hi, true);
-    q[p] = make_uint2((uint32_t)lo, (uint32_t)hi);
-    if (p + 1 < P) {
-      const v2f d0 = __builtin_amdgcn_cvt_pk_f32_fp8(lo, false), d1 = __builtin_amdgcn_cvt_pk_f32_fp8(lo, true);
-      const v2f d2 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), d3 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
-      const float d[8] = {d0.x, d0.y, d1.x, d1.y, d2.x, d2.y, d3.x, d3.y};
+    emit(p, make_uint2((uint32_t)lo, (uint32_t)hi));
+    // (v - digit) 32, exact
+    const v2f d0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((uint32_t)lo, 32.f, false), d1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((uint32_t)lo, 32.f, true);
+    const v2f d2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((uint32_t)hi, 32.f, false), d3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((uint32_t)hi, 32.f, true);
+    const float d[8] = {d0.x, d0.y, d1.x, d1.y, d2.x, d2.y, d3.x, d3.y};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (v[j] - d[j]) * 32.f;
-    }
+    for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(v[j], 32.f, -d[j]);
   }
   return (uint32_t)b;
 }
+
+// 16 bytes (a byte) per lane from base + voff + soff through a buffer of which
+// a negative voff is out of range: those lanes read zeros.  (Functions: the
+// host pass has no buffer descriptors.)
+RT_DEV v4i buffer_b128(const void *base, int voff, int soff) {
+  typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+  const auto buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, 0x7FFFFFFF, 0x00020000);
+  return __builtin_bit_cast(v4i, (v4u)__builtin_amdgcn_raw_buffer_load_b128(buf, voff, soff, 0));
+}
+RT_DEV uint32_t buffer_u8(const void *base, int voff, int soff) {
+  const auto buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, 0x7FFFFFFF, 0x00020000);
+  return (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(buf, voff, soff, 0);
+}
+constexpr int kOutOfRange = (int)0x80000000;
 
 // The elements of 2 and above of four e4m3 bytes (bit 6 is the exponent field's
 // top bit), the others zero.

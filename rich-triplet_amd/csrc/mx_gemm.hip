@@ -40,10 +40,7 @@ RT_DEV void split_group(const T *__restrict__ x, uint8_t *__restrict__ planes, u
                         size_t n8, uint32_t groups, int nk) {
   float v[8];
   load8(x + 8 * i, v);
-  uint2 q[P];
-  const uint32_t b = digits8<P>(v, q);
-#pragma unroll
-  for (int p = 0; p < P; ++p) reinterpret_cast<uint2 *>(planes + (size_t)p * 8 * n8)[i] = q[p];
+  const uint32_t b = digits8<P>(v, [&](int p, uint2 q) { reinterpret_cast<uint2 *>(planes + (size_t)p * 8 * n8)[i] = q; });
   if ((threadIdx.x & 3) == 0) {
     const size_t row = i / groups;
     const int kb = (int)(i - row * groups) >> 2;
@@ -214,13 +211,12 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
       __builtin_amdgcn_global_load_lds((gvoid *)scale_src(g.as, m0, g.M, BM, j), (lvoid *)(base + kAScale), 16, 0, 0);
     const uint8_t *ab = g.a + (size_t)p * g.plane + (size_t)m0 * arow;
     const int left = kb - 4 * j;  // blocks of the row from this stage on
-    constexpr int kOut = (int)0x80000000;
 #pragma unroll
     for (int i = 0; i < kWCopies; ++i)
-      copy_to_lds(wb, base + (kWCopies * wave + i) * 1024, wblk[i] < left ? (int)wo[i] : kOut, j * 64);
+      copy_to_lds(wb, base + (kWCopies * wave + i) * 1024, wblk[i] < left ? (int)wo[i] : kOutOfRange, j * 64);
 #pragma unroll
     for (int i = 0; i < kACopies; ++i)
-      copy_to_lds(ab, base + kWBytes + (kACopies * wave + i) * 1024, ablk[i] < left ? (int)ao[i] : kOut, j * kARow);
+      copy_to_lds(ab, base + kWBytes + (kACopies * wave + i) * 1024, ablk[i] < left ? (int)ao[i] : kOutOfRange, j * kARow);
   };
 
   // Fragments: row l16 of tile i is 16 rows further per tile, whole swizzle periods.

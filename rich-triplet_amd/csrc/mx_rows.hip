@@ -2,12 +2,11 @@
 // from memory to the matrix instructions once, through registers alone.
 //
 // A workgroup owns 16 RT weight rows, its waves share K in pieces (macros) of
-// 512.  Within a macro a lane takes the four blocks 4g .. 4g+3 of its row (g =
-// lane / 16) in four instructions, block 4g+s in instruction s: 64 contiguous
-// bytes per lane and one dword of scales, where the order of K would give each
-// instruction 64-byte pieces of rows.  The activations are the 16 CT columns of
-// the other operand: the digit planes of M rows (column m P + p: mx_gemm.hip
-// has the digits), or the rows themselves where they are microscaled.  The
+// 512: four instructions, each on 64 bytes of 16 rows and one scale byte per
+// block.  What lies past the end of a row reads as zeros, scale 2^-127.  The
+// activations are the 16 CT columns of the other operand: the digit planes of M
+// rows (column m P + p: mx_digits.hpp has the digits), or the rows themselves
+// where they are microscaled.  The
 // waves' sums, and the planes', are added through LDS in a fixed order.
 //
 // Three f32 rows (five bf16) fill one column tile, and each wave makes the
@@ -27,12 +26,12 @@ namespace rt {
 namespace {
 
 constexpr int kMacro = 512;  // elements of K in four instructions
-constexpr int kMaxWaves(int ct) { return ct == 1 ? 16 : ct == 2 ? 8 : 4; }  // also: sums in LDS stay within 64 KB
+constexpr int kMaxWaves(int ct) { return ct == 1 ? 10 : ct == 2 ? 8 : 4; }  // also: sums in LDS stay within 64 KB
 constexpr int kPitch = kMacro + 16;  // of a digit column in LDS: 16 columns of a read on disjoint banks
 constexpr int kScaleArea = 96;       // scale bytes of up to six rows
 constexpr int digit_area(int cols) { return cols * kPitch + kScaleArea; }  // of a wave
 
-enum Src { kF32, kBf16, kFp8, kFp4, kCols };  // kCols: digit columns in fragment order
+enum Src { kF32, kBf16, kFp8, kFp4, kCols5, kCols3 };  // kCols: digit columns in fragment order
 
 struct RowsArgs {
   const uint8_t *w, *wscale;
@@ -40,38 +39,21 @@ struct RowsArgs {
   const uint8_t *ascale;   // microscaled: [m][K/32]; digit columns: a dword per macro, tile and lane
   const float *bias;
   void *c;
-  int M, N, K, nmac, planes;
+  int M, N, K, nmac;
 };
-
-// Scale bytes of blocks b .. b+3 of a row of kb (b % 4 == 0); past its end 127.
-RT_DEV uint32_t scale_dword(const uint8_t *row, int b, int kb) {
-  if ((kb & 3) == 0) return b < kb ? *reinterpret_cast<const uint32_t *>(row + b) : 0x7F7F7F7Fu;
-  uint32_t v = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v |= (b + i < kb ? (uint32_t)row[b + i] : 127u) << (8 * i);
-  return v;
-}
-
-RT_DEV v4i load_block(const uint8_t *p, bool in) { return in ? *reinterpret_cast<const v4i *>(p) : (v4i){0, 0, 0, 0}; }
-RT_DEV v4i load_block_nt(const uint8_t *p, bool in) {
-  return in ? __builtin_nontemporal_load(reinterpret_cast<const v4i *>(p)) : (v4i){0, 0, 0, 0};
-}
 
 template <int SRC, bool TWO, int RT, int CT, class C>
 __global__ __launch_bounds__(64 * kMaxWaves(CT)) void k_mx_rows(RowsArgs g) {
-  constexpr bool kOwnDigits = SRC == kF32 || SRC == kBf16, kNarrow = SRC == kFp4;
-  constexpr int P = SRC == kF32 ? kPlanesF32 : SRC == kBf16 ? kPlanesBf16 : 1;
+  constexpr bool kOwnDigits = SRC == kF32 || SRC == kBf16, kNarrow = SRC == kFp4, kCols = SRC == kCols5 || SRC == kCols3;
+  constexpr int P = SRC == kF32 || SRC == kCols5 ? kPlanesF32 : SRC == kBf16 || SRC == kCols3 ? kPlanesBf16 : 1;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = (int)threadIdx.x & 63, l16 = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = (int)blockDim.x >> 6;
   const int n0 = (int)blockIdx.x * 16 * RT, kb = g.K / 32;
-  const uint8_t *we[RT], *wsr[RT];
+  const uint8_t *we = g.w + (size_t)n0 * (g.K / 2), *ws = g.wscale + (size_t)n0 * kb;
+  int wo[RT];  // this lane's row of each tile
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const size_t r = (size_t)min(n0 + 16 * i + l16, g.N - 1);
-    we[i] = g.w + r * (g.K / 2);
-    wsr[i] = g.wscale + r * kb;
-  }
+  for (int i = 0; i < RT; ++i) wo[i] = min(16 * i + l16, g.N - 1 - n0);
   v4f acc[RT][CT];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -81,74 +63,75 @@ __global__ __launch_bounds__(64 * kMaxWaves(CT)) void k_mx_rows(RowsArgs g) {
   const int col = min(l16, g.M * P - 1), col_m = col / P, col_p = col % P;  // columns past the last are never added
 
   for (int t = wave; t < g.nmac; t += waves) {
-    const int b0 = 16 * t + 4 * grp;  // this lane's first block
+    const int b = 16 * t + grp;  // this lane's block in the first instruction, four further in each
+    // The scale bytes of a row's blocks b, b+4, b+8, b+12.
+    auto scales = [&](const uint8_t *s, int row) __attribute__((always_inline)) {
+      uint32_t v = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v |= buffer_u8(s, b + 4 * i < kb ? row * kb + grp + 4 * i : kOutOfRange, 16 * t) << (8 * i);
+      return v;
+    };
+    // Own rows first: their digits are made while the weight is on its way.
+    const int k0 = kMacro * t + 8 * lane;
+    auto own_row = [&](int m, float (&x)[8]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = 0.f;
+      if (k0 < g.K) {
+        if constexpr (SRC == kF32) load8(static_cast<const float *>(g.a) + (size_t)m * g.K + k0, x);
+        if constexpr (SRC == kBf16) load8(static_cast<const uint16_t *>(g.a) + (size_t)m * g.K + k0, x);
+      }
+    };
+    float x[8];
+    if constexpr (kOwnDigits) own_row(0, x);
     v4i wq[RT][4];
-    uint32_t ws[RT];
+    uint32_t wsc[RT], asc[CT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) wq[i][s] = load_block_nt(we[i] + (size_t)(b0 + s) * 16, b0 + s < kb);
-      ws[i] = scale_dword(wsr[i], b0, kb);
+      for (int s = 0; s < 4; ++s)
+        wq[i][s] = buffer_b128(we, b + 4 * s < kb ? wo[i] * (g.K / 2) + 16 * grp + 64 * s : kOutOfRange, 256 * t);
+      wsc[i] = scales(ws, wo[i]);
     }
-    uint32_t as[CT];
-    v4i own[kOwnDigits ? 4 : 1][2];
-    // the block that logical block (g / 2) or (2 + g / 2) of instruction s is
-    const int c0 = 16 * t + 4 * (grp >> 1), c1 = c0 + 8, half = 16 * (grp & 1);
     if constexpr (kOwnDigits) {
       for (int m = 0; m < g.M; ++m) {
-        float v[8] = {};
-        const int k0 = kMacro * t + 8 * lane;
-        if (k0 < g.K) {
-          if constexpr (SRC == kF32) load8(static_cast<const float *>(g.a) + (size_t)m * g.K + k0, v);
-          else load8(static_cast<const uint16_t *>(g.a) + (size_t)m * g.K + k0, v);
-        }
-        uint2 q[P];
-        const uint32_t b = digits8<P>(v, q);
-#pragma unroll
-        for (int p = 0; p < P; ++p) *reinterpret_cast<uint2 *>(dig + (m * P + p) * kPitch + 8 * lane) = q[p];
-        if ((lane & 3) == 0) dsc[m * 16 + (lane >> 2)] = (uint8_t)b;
+        if (m) own_row(m, x);
+        const uint32_t e = digits8<P>(x, [&](int p, uint2 q) { *reinterpret_cast<uint2 *>(dig + (m * P + p) * kPitch + 8 * lane) = q; });
+        // block 4s+j of the macro at [j][s]
+        if ((lane & 3) == 0) dsc[m * 16 + ((lane >> 2) & 3) * 4 + (lane >> 4)] = (uint8_t)e;
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      asc[0] = *reinterpret_cast<const uint32_t *>(dsc + col_m * 16 + 4 * grp) - 0x01010101u * kPlaneShift * col_p;  // no borrow: a byte is at least 20
+    } else if constexpr (kCols) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const uint8_t *d = dig + col * kPitch + half;
-        own[s][0] = *reinterpret_cast<const v4i *>(d + (4 * (grp >> 1) + s) * 32);
-        own[s][1] = *reinterpret_cast<const v4i *>(d + (4 * (grp >> 1) + 8 + s) * 32);
-      }
-      const uint32_t sc = *reinterpret_cast<const uint32_t *>(dsc + col_m * 16 + 4 * grp);
-      as[0] = sc - 0x01010101u * kPlaneShift * col_p;  // no borrow: a byte is at least 20
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      for (int j = 0; j < CT; ++j) asc[j] = reinterpret_cast<const uint32_t *>(g.ascale)[((size_t)t * CT + j) * 64 + lane];
     } else {
 #pragma unroll
-      for (int j = 0; j < CT; ++j) {
-        if constexpr (SRC == kCols) as[j] = reinterpret_cast<const uint32_t *>(g.ascale)[((size_t)t * CT + j) * 64 + lane];
-        else as[j] = scale_dword(g.ascale + (size_t)min(16 * j + l16, g.M - 1) * kb, b0, kb);
-      }
+      for (int j = 0; j < CT; ++j) asc[j] = scales(g.ascale, min(16 * j + l16, g.M - 1));
     }
     auto mul = [&](auto sc) __attribute__((always_inline)) {
       constexpr int s = decltype(sc)::value;
 #pragma unroll
       for (int j = 0; j < CT; ++j) {
-        v4i x, y = {0, 0, 0, 0};
+        v4i u, v = {0, 0, 0, 0};  // a lane's 32 e4m3 elements are two half blocks, 64 of K apart
         if constexpr (kOwnDigits) {
-          x = own[s][0], y = own[s][1];
-        } else if constexpr (SRC == kCols) {
+          const uint8_t *d = dig + col * kPitch + 128 * s + 16 * grp;
+          u = *reinterpret_cast<const v4i *>(d), v = *reinterpret_cast<const v4i *>(d + 64);
+        } else if constexpr (kCols) {
           const uint8_t *d = static_cast<const uint8_t *>(g.a) + (((size_t)t * CT + j) * 4 + s) * 2048 + lane * 16;
-          x = *reinterpret_cast<const v4i *>(d), y = *reinterpret_cast<const v4i *>(d + 1024);
+          u = *reinterpret_cast<const v4i *>(d), v = *reinterpret_cast<const v4i *>(d + 1024);
         } else {
-          const uint8_t *d = static_cast<const uint8_t *>(g.a) + (size_t)min(16 * j + l16, g.M - 1) * (kNarrow ? g.K / 2 : g.K);
+          const int row = min(16 * j + l16, g.M - 1);
           if constexpr (kNarrow) {
-            x = load_block(d + (size_t)(b0 + s) * 16, b0 + s < kb);
+            u = buffer_b128(g.a, b + 4 * s < kb ? row * (g.K / 2) + 16 * grp + 64 * s : kOutOfRange, 256 * t);
           } else {
-            x = load_block(d + (size_t)(c0 + s) * 32 + half, c0 + s < kb);
-            y = load_block(d + (size_t)(c1 + s) * 32 + half, c1 + s < kb);
+            const int first = 16 * t + 4 * s + (grp >> 1);
+            u = buffer_b128(g.a, first < kb ? row * g.K + 16 * grp + 128 * s : kOutOfRange, 512 * t);
+            v = buffer_b128(g.a, first + 2 < kb ? row * g.K + 16 * grp + 128 * s + 64 : kOutOfRange, 512 * t);
           }
         }
-        v8i bv = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, up = bv;
+        v8i bv = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]}, up = bv;
         if constexpr (TWO) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) up[i] = (int)fp8_upper((uint32_t)bv[i]), bv[i] ^= up[i];
@@ -157,8 +140,8 @@ __global__ __launch_bounds__(64 * kMaxWaves(CT)) void k_mx_rows(RowsArgs g) {
         for (int i = 0; i < RT; ++i) {
           const v8i wv = {wq[i][s][0], wq[i][s][1], wq[i][s][2], wq[i][s][3], 0, 0, 0, 0};
           if constexpr (TWO)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, up, acc[i][j], 4, 0, s, (int)ws[i], s, (int)as[j]);
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, bv, acc[i][j], 4, kNarrow ? 4 : 0, s, (int)ws[i], s, (int)as[j]);
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, up, acc[i][j], 4, 0, s, (int)wsc[i], s, (int)asc[j]);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, bv, acc[i][j], 4, kNarrow ? 4 : 0, s, (int)wsc[i], s, (int)asc[j]);
         }
       }
     };
@@ -166,6 +149,11 @@ __global__ __launch_bounds__(64 * kMaxWaves(CT)) void k_mx_rows(RowsArgs g) {
     mul(IntC<1>{});
     mul(IntC<2>{});
     mul(IntC<3>{});
+    if constexpr (kOwnDigits) {  // read before the next macro's digits are written
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
   }
 
   // [wave][tile][lane] of four weight rows each
@@ -177,15 +165,16 @@ __global__ __launch_bounds__(64 * kMaxWaves(CT)) void k_mx_rows(RowsArgs g) {
     for (int j = 0; j < CT; ++j)
       *reinterpret_cast<v4f *>(red + (((wave * RT + i) * CT + j) * 64 + lane) * 4) = acc[i][j];
   __syncthreads();
-  const int planes = SRC == kCols ? g.planes : P;
   for (int o = (int)threadIdx.x; o < 16 * RT * g.M; o += (int)blockDim.x) {
     const int r = o % (16 * RT), m = o / (16 * RT), n = n0 + r;
     if (n >= g.N) continue;
     float v = 0.f;
+#pragma unroll 4
     for (int w = 0; w < waves; ++w)
-      for (int p = 0; p < planes; ++p) {
-        const int col = m * planes + p;
-        v += red[(((w * RT + (r >> 4)) * CT + (col >> 4)) * 64 + ((r >> 2) & 3) * 16 + (col & 15)) * 4 + (r & 3)];
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const int at = m * P + p;
+        v += red[(((w * RT + (r >> 4)) * CT + (at >> 4)) * 64 + ((r >> 2) & 3) * 16 + (at & 15)) * 4 + (r & 3)];
       }
     if (g.bias) v += g.bias[n];
     if constexpr (sizeof(C) == 4) static_cast<float *>(g.c)[(size_t)m * g.N + n] = v;
@@ -193,7 +182,7 @@ __global__ __launch_bounds__(64 * kMaxWaves(CT)) void k_mx_rows(RowsArgs g) {
   }
 }
 
-// Digit columns of M rows for k_mx_rows<kCols>: [macro][column tile][instruction][half][lane][16],
+// Digit columns of M rows for k_mx_rows<kCols*>: [macro][column tile][instruction][half][lane][16],
 // scales a dword per [macro][column tile][lane].  K is filled up to whole macros
 // with zeros; columns past M P are left as they are (they reach no output).
 template <class T, int P>
@@ -204,18 +193,18 @@ __global__ __launch_bounds__(256) void k_mx_split_cols(const T *__restrict__ x, 
   const int m = i / per_row, k0 = 8 * (i - m * per_row);
   float v[8] = {};
   if (k0 < K) load8(x + (size_t)m * K + k0, v);
-  uint2 q[P];
-  const uint32_t b = digits8<P>(v, q);
-  const int t = k0 / kMacro, blk = (k0 % kMacro) / 32, j = blk >> 2, s = blk & 3;
+  const int t = k0 / kMacro, blk = (k0 % kMacro) / 32, s = blk >> 2, j = blk & 3;
   const int g = (j & 1) * 2 + ((k0 >> 4) & 1), h = j >> 1;
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
+  const uint32_t b = digits8<P>(v, [&](int p, uint2 q) {
     const int col = m * P + p;
-    const size_t tile = (size_t)t * CT + (col >> 4);
-    *reinterpret_cast<uint2 *>(cols + ((tile * 4 + s) * 2 + h) * 1024 + (g * 16 + (col & 15)) * 16 + (k0 & 8)) = q[p];
-    // the lane of logical block j carries its scales
-    if ((k0 & 31) == 0) scales[(tile * 64 + j * 16 + (col & 15)) * 4 + s] = (uint8_t)(b == 255 ? 255 : b - kPlaneShift * p);
-  }
+    *reinterpret_cast<uint2 *>(cols + ((((size_t)t * CT + (col >> 4)) * 4 + s) * 2 + h) * 1024 + (g * 16 + (col & 15)) * 16 + (k0 & 8)) = q;
+  });
+  // the lane of logical block j carries its scales
+  if ((k0 & 31) == 0)
+    for (int p = 0; p < P; ++p) {
+      const int col = m * P + p;
+      scales[(((size_t)t * CT + (col >> 4)) * 64 + j * 16 + (col & 15)) * 4 + s] = (uint8_t)(b == 255 ? 255 : b - kPlaneShift * p);
+    }
 }
 
 size_t r256(size_t b) { return (b + 255) & ~size_t(255); }
@@ -231,14 +220,12 @@ RowsPlan rows_plan(MxAct act, int m, int n, int k) {
   if (cols > 64) return p;
   p.ok = true;
   p.ct = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
-  p.rt = p.ct;
+  // more weight rows per workgroup while that leaves one for every CU
+  for (p.rt = 1; p.rt < p.ct && (n + 32 * p.rt - 1) / (32 * p.rt) >= 256; p.rt *= 2) {}
   p.split = planes > 1 && p.ct > 1;
   const int nmac = (k + kMacro - 1) / kMacro;
-  const int64_t wgs = (n + 16 * p.rt - 1) / (16 * p.rt);
-  // about 16 waves per CU; then as few as give the same number of macros per wave
-  int cap = std::min(nmac, kMaxWaves(p.ct));
-  if (planes > 1 && !p.split) cap = std::min(cap, 65536 / digit_area((int)cols));
-  const int w = (int)std::min<int64_t>(cap, std::max<int64_t>((4096 + wgs - 1) / wgs, 4));
+  int w = std::min(nmac, kMaxWaves(p.ct));
+  if (planes > 1 && !p.split) w = std::min(w, 65536 / digit_area((int)cols));
   const int per = (nmac + w - 1) / w;
   p.waves = (nmac + per - 1) / per;
   return p;
@@ -253,7 +240,9 @@ hipError_t rows_launch(const RowsPlan &p, const RowsArgs &g, hipStream_t s) {
   const size_t lds = std::max(red, dig);  // at most 64 KB
   void (*kern)(RowsArgs) = nullptr;
   if constexpr (SRC == kF32 || SRC == kBf16) kern = k_mx_rows<SRC, TWO, 1, 1, C>;
-  else kern = p.ct == 1 ? k_mx_rows<SRC, TWO, 1, 1, C> : p.ct == 2 ? k_mx_rows<SRC, TWO, 2, 2, C> : k_mx_rows<SRC, TWO, 4, 4, C>;
+  else if (p.ct == 1) kern = k_mx_rows<SRC, TWO, 1, 1, C>;
+  else if (p.ct == 2) kern = p.rt == 1 ? k_mx_rows<SRC, TWO, 1, 2, C> : k_mx_rows<SRC, TWO, 2, 2, C>;
+  else kern = p.rt == 1 ? k_mx_rows<SRC, TWO, 1, 4, C> : p.rt == 2 ? k_mx_rows<SRC, TWO, 2, 4, C> : k_mx_rows<SRC, TWO, 4, 4, C>;
   hipLaunchKernelGGL(kern, grid, block, lds, s, g);
   return hipGetLastError();
 }
@@ -273,7 +262,7 @@ hipError_t launch_mx_rows(MxAct act, const void *a, const void *w, const float *
   const RowsPlan p = rows_plan(act, m, n, k);
   const int nmac = (k + kMacro - 1) / kMacro;
   const uint8_t *we = static_cast<const uint8_t *>(w), *ae = static_cast<const uint8_t *>(a);
-  RowsArgs g{we, we + (size_t)n * k / 2, a, nullptr, bias, c, m, n, k, nmac, 1};
+  RowsArgs g{we, we + (size_t)n * k / 2, a, nullptr, bias, c, m, n, k, nmac};
   if (p.split) {
     uint8_t *cols = static_cast<uint8_t *>(ws), *sc = cols + r256((size_t)nmac * p.ct * 8192);
     const dim3 grid((unsigned)(((int64_t)m * nmac * (kMacro / 8) + 255) / 256)), block(256);
@@ -283,8 +272,8 @@ hipError_t launch_mx_rows(MxAct act, const void *a, const void *w, const float *
       hipLaunchKernelGGL((k_mx_split_cols<uint16_t, kPlanesBf16>), grid, block, 0, s, static_cast<const uint16_t *>(a), cols, sc, m, k, nmac, p.ct);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    g.a = cols, g.ascale = sc, g.planes = act == kMxActF32 ? kPlanesF32 : kPlanesBf16;
-    return rows_launch<kCols, false, float>(p, g, s);
+    g.a = cols, g.ascale = sc;
+    return act == kMxActF32 ? rows_launch<kCols5, false, float>(p, g, s) : rows_launch<kCols3, false, float>(p, g, s);
   }
   switch (act) {
     case kMxActF32: return rows_launch<kF32, false, float>(p, g, s);
