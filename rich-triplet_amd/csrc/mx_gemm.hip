@@ -103,14 +103,15 @@ RT_DEV uint32_t lds_b32(uint32_t a) {
   asm volatile("ds_read_b32 %0, %1" : "=v"(v) : "v"(a));
   return v;
 }
-// Waits until at most N LDS operations are outstanding; the operands' readers come after it.
-template <int N>
-RT_DEV void lds_wait_n(u32x4 &v) {
-  asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(v) : "n"(N));
+RT_DEV uint32_t lds_u16(uint32_t a) {
+  uint32_t v;
+  asm volatile("ds_read_u16 %0, %1" : "=v"(v) : "v"(a));
+  return v;
 }
-template <int N>
-RT_DEV void lds_wait_n(uint32_t &v) {
-  asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(v) : "n"(N));
+// Waits for all LDS reads; the operand's readers come after it.
+template <class T>
+RT_DEV void lds_done(T &v) {
+  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(v));
 }
 
 template <int N, class F, int I = 0>
@@ -136,22 +137,72 @@ struct TileArgs {
   const float *bias;
   void *c;      // the result, or (ksplit > 1) the f32 partials [ksplit][M][N]
   int M, N, K, nk, planes, tiles_m, tiles_n, ksplit;
-  bool vec;  // 16-byte (bf16: 8-byte) stores of four columns
+  bool vec;  // rows of c are whole aligned 16-byte pieces
 };
 
+// Stores a wave's 16 MT x 16 NT of c; `stage` is LDS that only this wave uses.
+template <class C, int NT, int MT>
+RT_DEV void store_tile(const v4f (&acc)[NT][MT], uint8_t *stage, C *c, const float *bias, int row0, int col0, int M, int N,
+                       bool vec) {
+  constexpr int kRow = 16 * NT * (int)sizeof(C), kPitch = kRow + 16;  // the pad keeps rows off each other's banks
+  constexpr int kPer = 16 / (int)sizeof(C), kLanes = kRow / 16, kRows = 64 / kLanes;
+  const int lane = (int)threadIdx.x & 63, l16 = lane & 15, grp = lane >> 4;
+  v4f bv[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) bv[i][t] = bias ? bias[min(col0 + 16 * i + 4 * grp + t, N - 1)] : 0.f;
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const v4f v = acc[i][j] + bv[i];
+      uint8_t *d = stage + l16 * kPitch + (16 * i + 4 * grp) * sizeof(C);
+      if constexpr (sizeof(C) == 4) *reinterpret_cast<v4f *>(d) = v;
+      else *reinterpret_cast<uint2 *>(d) = make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int q = 0; q < 16 / kRows; ++q) {
+      const int r = q * kRows + lane / kLanes, row = row0 + 16 * j + r, col = col0 + (lane % kLanes) * kPer;
+      const u32x4 v = *reinterpret_cast<const u32x4 *>(stage + r * kPitch + (lane % kLanes) * 16);
+      if (row < M && col < N) {
+        C *d = c + (size_t)row * N + col;
+        if (vec) {  // N is whole 16-byte pieces
+          __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(d));
+        } else {
+#pragma unroll
+          for (int t = 0; t < kPer; ++t)
+            if (col + t < N) {
+              if constexpr (sizeof(C) == 4) d[t] = bits_f32(v[t]);
+              else d[t] = (C)(v[t / 2] >> (16 * (t & 1)));
+            }
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+
 // C tile of 16 NT WN columns (n) by 16 MT WM rows (m) by WN x WM waves, K in
-// stages of 128 through three LDS slots: while a stage is multiplied the copies
-// of the next two are on their way, one barrier per stage.
+// stages of 128 through three LDS slots.  While the fragments of stage u are
+// multiplied, those of u+1 are read into the wave's other set of registers and
+// the copies of u+2 and u+3 are on their way; one barrier per stage.
 //
 // A slot row is a row's 64 (e2m1) or 128 (e4m3) bytes of the stage, in 16-byte
-// units; unit u of row r lies at u ^ (r / 4 % 4) or u ^ (r / 2 % 8), so that the 16
-// rows of a fragment read hit 16 different bank groups.  Past the end of K the
+// units; unit u of row r lies at u ^ (r / 2 % 4) or u ^ (r / 2 % 8): the rows that
+// a fragment read takes at once then lie on different banks (r / 4 % 4 took
+// twice the cycles per read).  Past the end of K the
 // copies read out of their buffer's range, which leaves zeros in LDS.
 template <int FA, bool TWO, int WN, int WM, int NT, int MT, class C>
 __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
   constexpr int kWaves = WN * WM, BN = 16 * NT * WN, BM = 16 * MT * WM;
   constexpr int kARow = FA == kMxFp8 ? 128 : 64, kWBytes = BN * 64, kABytes = BM * kARow;
-  constexpr int kWScale = kWBytes + kABytes, kAScale = kWScale + BN * 4, kSlot = kAScale + BM * 4;
+  constexpr int kWScale = kWBytes + kABytes, kAScale = kWScale + 512 * ((BN + 127) / 128), kSlot = kAScale + 512 * ((BM + 127) / 128);
   constexpr int kWCopies = kWBytes / 1024 / kWaves, kACopies = kABytes / 1024 / kWaves;
   static_assert(kWBytes % (1024 * kWaves) == 0 && kABytes % (1024 * kWaves) == 0, "whole copies per wave");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[3 * kSlot];
@@ -178,7 +229,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
   int wblk[kWCopies], ablk[kACopies];
 #pragma unroll
   for (int i = 0; i < kWCopies; ++i) {
-    const int r = 16 * (kWCopies * wave + i) + (lane >> 2), u = wslot ^ ((r >> 2) & 3);
+    const int r = 16 * (kWCopies * wave + i) + (lane >> 2), u = wslot ^ ((r >> 1) & 3);
     wo[i] = (uint32_t)(min(n0 + r, g.N - 1) - n0) * (uint32_t)wrow + 16 * u;
     wblk[i] = u;
   }
@@ -189,7 +240,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
       ao[i] = (uint32_t)(min(m0 + r, g.M - 1) - m0) * (uint32_t)arow + 16 * u;
       ablk[i] = u >> 1;
     } else {
-      const int r = 16 * (kACopies * wave + i) + (lane >> 2), u = (lane & 3) ^ ((r >> 2) & 3);
+      const int r = 16 * (kACopies * wave + i) + (lane >> 2), u = (lane & 3) ^ ((r >> 1) & 3);
       ao[i] = (uint32_t)(min(m0 + r, g.M - 1) - m0) * (uint32_t)arow + 16 * u;
       ablk[i] = u;
     }
@@ -202,8 +253,11 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
     const int blk = min((row0 >> 7) + (tile_rows == 256 ? sh : 0), last);
     return s + ((size_t)blk * g.nk + j) * 512 + 16 * sl;
   };
-  auto issue = [&](int u, int slot) __attribute__((always_inline)) {
-    const int j = g.planes == 1 ? u : u / g.planes, p = u - j * g.planes;  // a weight's stage is read for all planes in turn
+  // The stage to copy next, u = j planes + p: a weight's stage serves all planes in turn.
+  int nj = u0 / g.planes, np = u0 - nj * g.planes, cp = np;
+  auto issue = [&](int slot) __attribute__((always_inline)) {
+    const int j = nj, p = np;
+    if (++np == g.planes) np = 0, ++nj;
     uint8_t *base = lds + slot * kSlot;
     if (wave == 0 && (BN == 256 || lane < 32))
       __builtin_amdgcn_global_load_lds((gvoid *)scale_src(g.ws, n0, g.N, BN, j), (lvoid *)(base + kWScale), 16, 0, 0);
@@ -221,9 +275,9 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
 
   // Fragments: row l16 of tile i is 16 rows further per tile, whole swizzle periods.
   const uint32_t lb = lds_addr(lds);
-  const uint32_t fw = lb + (16 * NT * wn + l16) * 64 + 16 * (grp ^ ((l16 >> 2) & 3));
+  const uint32_t fw = lb + (16 * NT * wn + l16) * 64 + 16 * (grp ^ ((l16 >> 1) & 3));
   const uint32_t fa0 = lb + kWBytes + (16 * MT * wm + l16) * kARow +
-                       16 * (FA == kMxFp8 ? grp ^ ((l16 >> 1) & 7) : grp ^ ((l16 >> 2) & 3));
+                       16 * (FA == kMxFp8 ? grp ^ ((l16 >> 1) & 7) : grp ^ ((l16 >> 1) & 3));
   const uint32_t fa1 = lb + kWBytes + (16 * MT * wm + l16) * kARow + 16 * ((4 + grp) ^ ((l16 >> 1) & 7));
   // a lane's scale bytes: [128 rows][64 lanes][8 tiles]
   const uint32_t fws = lb + kWScale + (NT * wn / 8) * 512 + lane * 8 + (NT * wn) % 8;
@@ -235,54 +289,54 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
 
-  if (u0 < u1) issue(u0, 0);
-  if (u0 + 1 < u1) issue(u0 + 1, 1);
-  int slot = 0;
-  for (int u = u0; u < u1; ++u) {
-    // this wave's copies of stage u (those of u+1 may be on their way), then everyone's
-    if (u + 1 < u1) wait_vmcnt<kWCopies + kACopies>();
-    else wait_vmcnt<0>();
-    wg_barrier();
-    // the slot of stage u+2 was read in stage u-1, by every wave before this barrier
-    if (u + 2 < u1) issue(u + 2, slot == 0 ? 2 : slot - 1);
-    __builtin_amdgcn_sched_barrier(0);
+  constexpr int kUnits = FA == kMxFp8 ? 2 : 1;
+  struct Frag {
+    u32x4 w[NT], a[MT][kUnits];
+    uint32_t sw[NT / 4], sa[(MT + 3) / 4];
+  };
+  auto read = [&](Frag &f, int slot) __attribute__((always_inline)) {
     const uint32_t so = (uint32_t)slot * kSlot;
-    uint32_t sw[NT / 4], sa[MT / 4];
-    u32x4 wf[NT], af[MT][FA == kMxFp8 ? 2 : 1];
 #pragma unroll
-    for (int i = 0; i < NT / 4; ++i) sw[i] = lds_b32(fws + so + 4 * i);
+    for (int i = 0; i < NT / 4; ++i) f.sw[i] = lds_b32(fws + so + 4 * i);
+    if constexpr (MT == 2) f.sa[0] = lds_u16(fas + so);
+    else
 #pragma unroll
-    for (int i = 0; i < MT / 4; ++i) sa[i] = lds_b32(fas + so + 4 * i);
-    steps<NT>([&](auto ic) __attribute__((always_inline)) {
-      constexpr int i = decltype(ic)::value;
-      wf[i] = lds_b128<i * 1024>(fw + so);
-    });
+      for (int i = 0; i < MT / 4; ++i) f.sa[i] = lds_b32(fas + so + 4 * i);
     steps<MT>([&](auto jc) __attribute__((always_inline)) {
       constexpr int j = decltype(jc)::value;
-      af[j][0] = lds_b128<j * 16 * kARow>(fa0 + so);
-      if constexpr (FA == kMxFp8) af[j][1] = lds_b128<j * 16 * kARow>(fa1 + so);
+      f.a[j][0] = lds_b128<j * 16 * kARow>(fa0 + so);
+      if constexpr (kUnits == 2) f.a[j][1] = lds_b128<j * 16 * kARow>(fa1 + so);
     });
-    constexpr int kPerM = FA == kMxFp8 ? 2 : 1;
-    lds_wait_n<MT * kPerM>(sw[0]);
+    steps<NT>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value;
+      f.w[i] = lds_b128<i * 1024>(fw + so);
+    });
+  };
+  auto done = [&](Frag &f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < NT / 4; ++i) lds_wait_n<MT * kPerM>(sw[i]);
+    for (int i = 0; i < NT / 4; ++i) lds_done(f.sw[i]);
 #pragma unroll
-    for (int i = 0; i < MT / 4; ++i) lds_wait_n<MT * kPerM>(sa[i]);
+    for (int i = 0; i < (MT + 3) / 4; ++i) lds_done(f.sa[i]);
 #pragma unroll
-    for (int i = 0; i < NT; ++i) lds_wait_n<MT * kPerM>(wf[i]);
+    for (int i = 0; i < NT; ++i) lds_done(f.w[i]);
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int t = 0; t < kUnits; ++t) lds_done(f.a[j][t]);
+  };
+  auto multiply = [&](Frag &f) __attribute__((always_inline)) {
     if (g.planes > 1) {
-      const uint32_t less = 0x01010101u * kPlaneShift * (uint32_t)(u % g.planes);
+      const uint32_t less = 0x01010101u * kPlaneShift * (uint32_t)cp;
 #pragma unroll
-      for (int i = 0; i < MT / 4; ++i) sa[i] -= less;  // no borrow: a digit block's byte is at least 20
+      for (int i = 0; i < (MT + 3) / 4; ++i) f.sa[i] -= less;  // no borrow: a digit block's byte is at least 20
+      cp = cp + 1 == g.planes ? 0 : cp + 1;
     }
     steps<MT>([&](auto jc) __attribute__((always_inline)) {
-      constexpr int j = decltype(jc)::value, kLeft = (MT - 1 - j) * kPerM;
+      constexpr int j = decltype(jc)::value;
+      v8i av = {(int)f.a[j][0][0], (int)f.a[j][0][1], (int)f.a[j][0][2], (int)f.a[j][0][3], 0, 0, 0, 0};
+      if constexpr (kUnits == 2)
 #pragma unroll
-      for (int t = 0; t < kPerM; ++t) lds_wait_n<kLeft>(af[j][t]);
-      v8i av = {(int)af[j][0][0], (int)af[j][0][1], (int)af[j][0][2], (int)af[j][0][3], 0, 0, 0, 0};
-      if constexpr (FA == kMxFp8)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) av[4 + t] = (int)af[j][1][t];
+        for (int t = 0; t < 4; ++t) av[4 + t] = (int)f.a[j][1][t];
       v8i up = av;
       if constexpr (TWO) {
 #pragma unroll
@@ -290,56 +344,57 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
       }
       steps<NT>([&](auto ic) __attribute__((always_inline)) {
         constexpr int i = decltype(ic)::value;
-        const v8i wv = {(int)wf[i][0], (int)wf[i][1], (int)wf[i][2], (int)wf[i][3], 0, 0, 0, 0};
+        const v8i wv = {(int)f.w[i][0], (int)f.w[i][1], (int)f.w[i][2], (int)f.w[i][3], 0, 0, 0, 0};
         if constexpr (TWO)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, up, acc[i][j], 4, 0, i & 3, (int)sw[i / 4],
-                                                                       j & 3, (int)sa[j / 4]);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, up, acc[i][j], 4, 0, i & 3, (int)f.sw[i / 4],
+                                                                       j & 3, (int)f.sa[j / 4]);
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, av, acc[i][j], 4, FA == kMxFp8 ? 0 : 4, i & 3,
-                                                                     (int)sw[i / 4], j & 3, (int)sa[j / 4]);
+                                                                     (int)f.sw[i / 4], j & 3, (int)f.sa[j / 4]);
       });
     });
-    slot = slot == 2 ? 0 : slot + 1;
+  };
+
+  // Waits count this wave's copies of whole stages; waves 0 and 1 issue one more
+  // (scales), the first of its stage, so they wait for at least as much.
+  constexpr int kCopies = kWCopies + kACopies;
+  const int n = u1 - u0;
+  issue(0);
+  if (n > 1) issue(1);
+  if (n > 2) issue(2);
+  if (n > 2) wait_vmcnt<2 * kCopies>();
+  else if (n > 1) wait_vmcnt<kCopies>();
+  else wait_vmcnt<0>();
+  wg_barrier();
+  Frag f0, f1;
+  read(f0, 0);
+  int slot = 0;
+  auto stage = [&](Frag &cur, Frag &nxt, int u) __attribute__((always_inline)) {
+    done(cur);
+    if (u + 1 < n) {
+      if (u + 2 < n) wait_vmcnt<kCopies>();
+      else wait_vmcnt<0>();
+      // every wave has read stage u and has its copies of stage u+1
+      wg_barrier();
+      if (u + 3 < n) issue(slot);
+      slot = slot == 2 ? 0 : slot + 1;
+      read(nxt, slot);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(cur);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int u = 0; u < n; u += 2) {
+    stage(f0, f1, u);
+    if (u + 1 < n) stage(f1, f0, u + 1);
   }
 
-  // Lane: columns 4 grp .. + 3 of each 16, row l16.
-  const bool part = g.ksplit > 1;
-#pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const int row = m0 + 16 * (MT * wm + j) + l16;
-    if (row >= g.M) continue;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int col = n0 + 16 * (NT * wn + i) + 4 * grp;
-      if (col >= g.N) continue;
-      v4f v = acc[i][j];
-      if (part) {
-        float *d = static_cast<float *>(g.c) + ((size_t)split * g.M + row) * g.N + col;
-        if (g.vec) *reinterpret_cast<v4f *>(d) = v;
-        else
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            if (col + t < g.N) d[t] = v[t];
-        continue;
-      }
-      if (g.bias)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) v[t] += g.bias[min(col + t, g.N - 1)];
-      C *d = static_cast<C *>(g.c) + (size_t)row * g.N + col;
-      if constexpr (sizeof(C) == 4) {
-        if (g.vec) *reinterpret_cast<v4f *>(d) = v;
-        else
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            if (col + t < g.N) d[t] = v[t];
-      } else {
-        if (g.vec) *reinterpret_cast<uint2 *>(d) = make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
-        else
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            if (col + t < g.N) d[t] = f32_to_bf16_bits(v[t]);
-      }
-    }
-  }
+  // A lane holds columns 4 grp .. + 3 of each 16, row l16.  16 rows at a time go
+  // through this wave's part of LDS and leave as whole row pieces, 16 bytes per lane.
+  if (n > 0) wg_barrier();  // other waves' last reads
+  if (g.ksplit > 1) store_tile<float>(acc, lds + wave * (3 * kSlot / kWaves), static_cast<float *>(g.c) + (size_t)split * g.M * g.N,
+                                      nullptr, m0 + 16 * MT * wm, n0 + 16 * NT * wn, g.M, g.N, g.vec);
+  else store_tile<C>(acc, lds + wave * (3 * kSlot / kWaves), static_cast<C *>(g.c), g.bias, m0 + 16 * MT * wm,
+                     n0 + 16 * NT * wn, g.M, g.N, g.vec);
 }
 
 // c[m][n] = sum over the K splits, in their order, + bias; V columns per thread.
@@ -380,23 +435,34 @@ size_t r256(size_t b) { return (b + 255) & ~size_t(255); }
 int planes_of(MxAct act) { return act == kMxActF32 ? kPlanesF32 : act == kMxActBf16 ? kPlanesBf16 : 1; }
 bool digits(MxAct act) { return act == kMxActF32 || act == kMxActBf16; }
 
+// C tiles: rows (m) by columns (n).
+enum Tile { k64x128, k128x128, k256x256, k128x256 };
+constexpr int tile_m(int t) { return t == k64x128 ? 64 : t == k256x256 ? 256 : 128; }
+constexpr int tile_n(int t) { return t == k256x256 || t == k128x256 ? 256 : 128; }
+
 struct Plan {
-  int tile, ksplit;  // rows and columns of a C tile
+  int tile, ksplit;
 };
 Plan plan_for(MxAct act, int m, int n, int k) {
-  const int64_t t256 = (int64_t)((m + 255) / 256) * ((n + 255) / 256), t128 = (int64_t)((m + 127) / 128) * ((n + 127) / 128);
+  const int64_t t256 = (int64_t)((m + 255) / 256) * ((n + 255) / 256);
   const int stages = planes_of(act) * ((k + 127) / 128);
-  if (t256 >= 256) return {256, 1};
-  int ks = (int)std::min<int64_t>(std::max<int64_t>(512 / t128, 1), 32);
+  if (t256 >= 256 && act == kMxActFp4) return {k128x256, 1};
+  if (t256 >= 256) return {k128x128, 1};
+  const int tile = m <= 64 ? k64x128 : k128x128;
+  const int64_t tiles = (int64_t)((m + tile_m(tile) - 1) / tile_m(tile)) * ((n + tile_n(tile) - 1) / tile_n(tile));
+  int ks = (int)std::min<int64_t>(std::max<int64_t>(512 / tiles, 1), 32);
   ks = std::min(ks, std::max(stages / 4, 1));
-  return {128, ks};
+  return {tile, ks};
 }
 
 template <int FA, bool TWO, class C>
 hipError_t tile_launch(const TileArgs &g, int tile, hipStream_t s) {
   const dim3 grid(g.tiles_m * g.tiles_n * g.ksplit);
-  auto kern = tile == 256 ? k_mx_gemm_tile<FA, TWO, 2, 4, 8, 4, C> : k_mx_gemm_tile<FA, TWO, 2, 2, 4, 4, C>;
-  hipLaunchKernelGGL(kern, grid, dim3(tile == 256 ? 512 : 256), 0, s, g);
+  auto kern = tile == k256x256   ? k_mx_gemm_tile<FA, TWO, 2, 4, 8, 4, C>
+              : tile == k128x256 ? k_mx_gemm_tile<FA, TWO, 2, 2, 8, 4, C>
+              : tile == k128x128 ? k_mx_gemm_tile<FA, TWO, 2, 2, 4, 4, C>
+                                 : k_mx_gemm_tile<FA, TWO, 2, 2, 4, 2, C>;
+  hipLaunchKernelGGL(kern, grid, dim3(tile == k256x256 ? 512 : 256), 0, s, g);
   return hipGetLastError();
 }
 
@@ -440,8 +506,8 @@ hipError_t launch_mx_gemm(MxAct act, const void *a, const void *w, const float *
   void *out = to_part ? static_cast<void *>(part) : c;
   const bool out16 = !to_part && c_bf16;
   const TileArgs g{digits(act) ? planes : ae, we, as, wsc, mk, to_part ? nullptr : bias, out, m, n, k, nk, planes_of(act),
-                   (m + plan.tile - 1) / plan.tile, (n + plan.tile - 1) / plan.tile, plan.ksplit,
-                   n % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (out16 ? 7 : 15)) == 0};
+                   (m + tile_m(plan.tile) - 1) / tile_m(plan.tile), (n + tile_n(plan.tile) - 1) / tile_n(plan.tile), plan.ksplit,
+                   n % (out16 ? 8 : 4) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0};
   if (act == kMxActFp4) e = out16 ? tile_launch<kMxFp4, false, uint16_t>(g, plan.tile, s) : tile_launch<kMxFp4, false, float>(g, plan.tile, s);
   else if (act == kMxActFp8 && !c_bf16) e = tile_launch<kMxFp8, true, float>(g, plan.tile, s);
   else e = out16 ? tile_launch<kMxFp8, false, uint16_t>(g, plan.tile, s) : tile_launch<kMxFp8, false, float>(g, plan.tile, s);
