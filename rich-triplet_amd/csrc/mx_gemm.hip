@@ -140,23 +140,22 @@ struct TileArgs {
   bool vec;  // rows of c are whole aligned 16-byte pieces
 };
 
-// Stores a wave's 16 MT x 16 NT of c; `stage` is LDS that only this wave uses.
-template <class C, int NT, int MT>
+// Stores column tiles I0 .. I0 + NI - 1 (columns from col0 on) of a wave's 16 MT
+// rows of c; `stage` is LDS that only this wave uses.
+template <class C, bool BIAS, int I0, int NI, int NT, int MT>
 RT_DEV void store_tile(const v4f (&acc)[NT][MT], uint8_t *stage, C *c, const float *bias, int row0, int col0, int M, int N,
                        bool vec) {
-  constexpr int kRow = 16 * NT * (int)sizeof(C), kPitch = kRow + 16;  // the pad keeps rows off each other's banks
+  constexpr int kRow = 16 * NI * (int)sizeof(C), kPitch = kRow + 16;  // the pad keeps rows off each other's banks
   constexpr int kPer = 16 / (int)sizeof(C), kLanes = kRow / 16, kRows = 64 / kLanes;
   const int lane = (int)threadIdx.x & 63, l16 = lane & 15, grp = lane >> 4;
-  v4f bv[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int t = 0; t < 4; ++t) bv[i][t] = bias ? bias[min(col0 + 16 * i + 4 * grp + t, N - 1)] : 0.f;
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const v4f v = acc[i][j] + bv[i];
+    for (int i = 0; i < NI; ++i) {
+      v4f v = acc[I0 + i][j];
+      if constexpr (BIAS)  // from the cache for each 16 rows: kept in registers, the wave's columns would cost 32
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[t] += bias[min(col0 + 16 * i + 4 * grp + t, N - 1)];
       uint8_t *d = stage + l16 * kPitch + (16 * i + 4 * grp) * sizeof(C);
       if constexpr (sizeof(C) == 4) *reinterpret_cast<v4f *>(d) = v;
       else *reinterpret_cast<uint2 *>(d) = make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
@@ -185,6 +184,7 @@ RT_DEV void store_tile(const v4f (&acc)[NT][MT], uint8_t *stage, C *c, const flo
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    __builtin_amdgcn_sched_barrier(0);  // the next rows' accumulators are not fetched early: registers
   }
 }
 
@@ -391,10 +391,192 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
   // A lane holds columns 4 grp .. + 3 of each 16, row l16.  16 rows at a time go
   // through this wave's part of LDS and leave as whole row pieces, 16 bytes per lane.
   if (n > 0) wg_barrier();  // other waves' last reads
-  if (g.ksplit > 1) store_tile<float>(acc, lds + wave * (3 * kSlot / kWaves), static_cast<float *>(g.c) + (size_t)split * g.M * g.N,
-                                      nullptr, m0 + 16 * MT * wm, n0 + 16 * NT * wn, g.M, g.N, g.vec);
-  else store_tile<C>(acc, lds + wave * (3 * kSlot / kWaves), static_cast<C *>(g.c), g.bias, m0 + 16 * MT * wm,
-                     n0 + 16 * NT * wn, g.M, g.N, g.vec);
+  uint8_t *buf = lds + wave * (3 * kSlot / kWaves);
+  const int row0 = m0 + 16 * MT * wm, col0 = n0 + 16 * NT * wn;
+  if (g.ksplit > 1)
+    store_tile<float, false, 0, NT>(acc, buf, static_cast<float *>(g.c) + (size_t)split * g.M * g.N, nullptr, row0, col0, g.M, g.N, g.vec);
+  else if (g.bias)
+    store_tile<C, true, 0, NT>(acc, buf, static_cast<C *>(g.c), g.bias, row0, col0, g.M, g.N, g.vec);
+  else
+    store_tile<C, false, 0, NT>(acc, buf, static_cast<C *>(g.c), nullptr, row0, col0, g.M, g.N, g.vec);
+}
+
+// The largest products of MXFP4 activations: 256 x 256 of c by four waves, one
+// on each SIMD, 128 x 128 each, whose fragments cost 16 bytes of LDS reads per
+// lane for four instructions (the smaller tiles' 64 x 128: for 2.7).
+//
+// K goes in chunks of 256, a row's whole cache line (a copy of half lines asks
+// the L2 for twice as many requests), two steps of 128 each, through two LDS
+// slots.  A step's 64 instructions run with the LDS reads of the next step's
+// fragments and, in the odd step, the next copies between them; there is one
+// barrier per chunk, at the start of its odd step: by then every wave has read
+// the whole chunk, and the next one's copies, issued a chunk earlier, have landed.
+//
+// A workgroup stays on its CU for several tiles, and the chunks of the next tile
+// follow those of the present one without a pause: its first fragments are in
+// registers before the accumulators are stored, and the stores drain under it.
+template <class C, bool BIAS>
+__global__ __launch_bounds__(256, 1) void k_mx_gemm_big(TileArgs g) {
+  constexpr int kOperand = 256 * 128, kScales = 4 * 1024, kSlot = 2 * kOperand + kScales, kStage = 6144;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kSlot + 4 * kStage];
+  static_assert(sizeof(lds) <= 160 * 1024, "LDS of a CU");
+  const int tid = (int)threadIdx.x, lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave & 1, wm = wave >> 1;
+  // XCD x8 gets a contiguous run of tiles [first, last), its workgroups (in turn) every `step`-th of them
+  const int items = g.tiles_m * g.tiles_n, x8 = (int)blockIdx.x & 7, r8 = items & 7, q8 = items >> 3;
+  const int first = x8 < r8 ? x8 * (q8 + 1) : r8 * (q8 + 1) + (x8 - r8) * q8, last = first + q8 + (x8 < r8 ? 1 : 0);
+  const int step = ((int)gridDim.x - x8 + 7) >> 3;
+  const int kb = g.K / 32, chunks = g.nk / 2;  // host: nk even, the scales of a last odd step's second half neutral
+  const size_t row_bytes = (size_t)g.K / 2;
+
+  // What a tile's copies go by.  Copy q of an operand: rows 8 (8 wave + q) + lane / 8, unit (lane % 8) of the slot row.
+  const int crow = 64 * wave + (lane >> 3), unit = (lane & 7) ^ ((crow >> 1) & 7);  // odd q: 8 rows on, 4 in the swizzle
+  struct Source {
+    const uint8_t *w, *a, *s;
+  };
+  auto corner = [&](int tile, int &m0, int &n0) __attribute__((always_inline)) {
+    const int group = tile / (8 * g.tiles_n), in_group = tile % (8 * g.tiles_n), gm = min(8, g.tiles_m - group * 8);
+    m0 = (group * 8 + in_group % gm) * 256, n0 = in_group / gm * 256;
+  };
+  uint32_t wo[8], ao[8];
+  auto source = [&](int tile) __attribute__((always_inline)) {
+    int m0, n0;
+    corner(tile, m0, n0);
+    Source t;
+    t.w = g.w + (size_t)n0 * row_bytes, t.a = g.a + (size_t)m0 * row_bytes;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      wo[q] = (uint32_t)min(crow + 8 * q, g.N - 1 - n0) * (uint32_t)row_bytes + 16 * (unit ^ (4 * (q & 1)));
+      ao[q] = (uint32_t)min(crow + 8 * q, g.M - 1 - m0) * (uint32_t)row_bytes + 16 * (unit ^ (4 * (q & 1)));
+    }
+    // scales: piece `wave` of a chunk: step wave / 2, the weight's (even) or the activations'
+    const int blk = min(((wave & 1 ? m0 : n0) >> 7) + (lane >> 5), ((wave & 1 ? g.M : g.N) - 1) >> 7);
+    t.s = (wave & 1 ? g.as : g.ws) + ((size_t)blk * g.nk + (wave >> 1)) * 512 + 16 * (lane & 31);
+    return t;
+  };
+  auto copy = [&](const Source &t, int c, int slot, auto qc) __attribute__((always_inline)) {  // 0 scales, 1..8 weight, 9..16 activations
+    constexpr int q = decltype(qc)::value;
+    uint8_t *base = lds + slot * kSlot;
+    if constexpr (q == 0) {
+      __builtin_amdgcn_global_load_lds((gvoid *)(t.s + (size_t)c * 1024), (lvoid *)(base + 2 * kOperand + wave * 1024), 16, 0, 0);
+    } else {
+      constexpr int r = (q - 1) & 7;
+      const bool in = 8 * c + (unit ^ (4 * (r & 1))) < kb;
+      if constexpr (q <= 8) copy_to_lds(t.w, base + (8 * wave + r) * 1024, in ? (int)wo[r] : kOutOfRange, c * 128);
+      else copy_to_lds(t.a, base + kOperand + (8 * wave + r) * 1024, in ? (int)ao[r] : kOutOfRange, c * 128);
+    }
+  };
+
+  struct Frag {
+    u32x4 w[8], a[8];
+    uint2 sw, sa;
+  };
+  const uint32_t lb = lds_addr(lds), swz = 16 * (grp ^ ((l16 >> 1) & 7));
+  const uint32_t rw = lb + (128 * wn + l16) * 128 + swz, ra = lb + kOperand + (128 * wm + l16) * 128 + swz;
+  const uint32_t rsw = lb + 2 * kOperand + wn * 512 + lane * 8, rsa = lb + 2 * kOperand + 1024 + wm * 512 + lane * 8;
+  auto read = [&](Frag &f, uint32_t so, auto hc, auto qc) __attribute__((always_inline)) {  // read q of step h: 0, 1 scales, then a, w
+    constexpr int h = decltype(hc)::value, q = decltype(qc)::value;
+    if constexpr (q == 0) asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(f.sw) : "v"(rsw + so), "n"(h * 2048));
+    else if constexpr (q == 1) asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(f.sa) : "v"(rsa + so), "n"(h * 2048));
+    else if constexpr (q < 10) f.a[q - 2] = lds_b128<(q - 2) * 2048>((ra ^ (64 * h)) + so);
+    else f.w[q - 10] = lds_b128<(q - 10) * 2048>((rw ^ (64 * h)) + so);
+  };
+  auto done = [&](Frag &f) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f.sw), "+v"(f.sa));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(f.w[i]), "+v"(f.a[i]));
+  };
+  v4f acc[8][8];
+  // Written out, for accumulators that stay where they are: the register
+  // allocator otherwise moves a third of them before every instruction.  Its
+  // operands come from LDS reads that done() has waited for, none from the VALU.
+  auto mfma = [&](Frag &f, auto zero, auto mc) __attribute__((always_inline)) {
+    constexpr int m = decltype(mc)::value, j = m >> 3, i = m & 7;
+    if constexpr (decltype(zero)::value)
+      asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, 0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
+                   : "=a"(acc[i][j])
+                   : "v"(f.w[i]), "v"(f.a[j]), "v"(i < 4 ? f.sw.x : f.sw.y), "v"(j < 4 ? f.sa.x : f.sa.y), "n"(i & 1),
+                     "n"(j & 1), "n"((i >> 1) & 1), "n"((j >> 1) & 1));
+    else
+      asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
+                   : "+a"(acc[i][j])
+                   : "v"(f.w[i]), "v"(f.a[j]), "v"(i < 4 ? f.sw.x : f.sw.y), "v"(j < 4 ? f.sa.x : f.sa.y), "n"(i & 1),
+                     "n"(j & 1), "n"((i >> 1) & 1), "n"((j >> 1) & 1));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  Frag f0, f1;
+  auto even = [&](auto zero, uint32_t here) __attribute__((always_inline)) {
+    done(f0);
+    __builtin_amdgcn_sched_barrier(0);
+    steps<64>([&](auto mc) __attribute__((always_inline)) {
+      constexpr int m = decltype(mc)::value;
+      mfma(f0, zero, mc);
+      if constexpr ((m & 1) && m / 2 < 18) read(f1, here, IntC<1>{}, IntC<m / 2>{});
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  bool stored = false;  // nothing but the last tile's kStores stores was issued after the copies that the step needs
+  constexpr int kStores = 128 * 128 * (int)sizeof(C) / 1024;
+  auto odd = [&](uint32_t there, const Source &t, int c, int slot) __attribute__((always_inline)) {
+    done(f1);
+    if (stored) wait_vmcnt<(kStores < 63 ? kStores : 63)>();
+    else wait_vmcnt<0>();  // this wave's copies of the next chunk
+    stored = false;
+    wg_barrier();                          // everyone's; and everyone has read this one
+    __builtin_amdgcn_sched_barrier(0);
+    steps<64>([&](auto mc) __attribute__((always_inline)) {
+      constexpr int m = decltype(mc)::value;
+      mfma(f1, IntC<0>{}, mc);
+      if constexpr ((m & 1) && m / 2 < 18) read(f0, there, IntC<0>{}, IntC<m / 2>{});
+      if constexpr (!(m & 1) && m / 2 < 17) copy(t, c, slot, IntC<m / 2>{});
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+
+  int tile = first + ((int)blockIdx.x >> 3);
+  if (tile >= last) return;  // host: no more workgroups than tiles; an XCD's run can be one shorter
+  Source src = source(tile);          // of the copies, which run ahead into the next tile
+  int ahead = tile, ac = 0, slot = 0;  // tile and chunk of the next copy; slot of the chunk being multiplied
+  auto advance = [&]() __attribute__((always_inline)) {  // past the last tile the copies repeat it, unused
+    if (++ac < chunks) return;
+    ac = 0;
+    if (ahead + step < last) ahead += step, src = source(ahead);
+  };
+  steps<17>([&](auto q) { copy(src, ac, 0, q); });
+  advance();
+  steps<17>([&](auto q) { copy(src, ac, 1, q); });
+  advance();
+  wait_vmcnt<17>();
+  wg_barrier();
+  steps<18>([&](auto q) { read(f0, 0, IntC<0>{}, q); });
+  for (;;) {
+    even(IntC<1>{}, slot * kSlot);
+    odd((slot ^ 1) * kSlot, src, ac, slot);
+    advance();
+    slot ^= 1;
+    for (int c = 1; c < chunks; ++c) {
+      even(IntC<0>{}, slot * kSlot);
+      odd((slot ^ 1) * kSlot, src, ac, slot);
+      advance();
+      slot ^= 1;
+    }
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last results, before anything reads them
+    uint8_t *stage = lds + 2 * kSlot + wave * kStage;
+    int m0, n0;
+    corner(tile, m0, n0);
+    stored = g.vec && m0 + 256 <= g.M && n0 + 256 <= g.N;  // every store of the tile is issued
+    m0 += 128 * wm, n0 += 128 * wn;
+    if constexpr (sizeof(C) == 2) {
+      store_tile<C, BIAS, 0, 8>(acc, stage, static_cast<C *>(g.c), g.bias, m0, n0, g.M, g.N, g.vec);
+    } else {
+      store_tile<C, BIAS, 0, 4>(acc, stage, static_cast<C *>(g.c), g.bias, m0, n0, g.M, g.N, g.vec);
+      store_tile<C, BIAS, 4, 4>(acc, stage, static_cast<C *>(g.c), g.bias, m0, n0 + 64, g.M, g.N, g.vec);
+    }
+    tile += step;
+    if (tile >= last) break;
+  }
+  done(f0);
+  wait_vmcnt<0>();  // the copies that ran ahead
 }
 
 // c[m][n] = sum over the K splits, in their order, + bias; V columns per thread.
@@ -436,9 +618,9 @@ int planes_of(MxAct act) { return act == kMxActF32 ? kPlanesF32 : act == kMxActB
 bool digits(MxAct act) { return act == kMxActF32 || act == kMxActBf16; }
 
 // C tiles: rows (m) by columns (n).
-enum Tile { k64x128, k128x128, k256x256, k128x256 };
-constexpr int tile_m(int t) { return t == k64x128 ? 64 : t == k256x256 ? 256 : 128; }
-constexpr int tile_n(int t) { return t == k256x256 || t == k128x256 ? 256 : 128; }
+enum Tile { k64x128, k128x128, k256x256, k128x256, kBig };
+constexpr int tile_m(int t) { return t == k64x128 ? 64 : t == k256x256 || t == kBig ? 256 : 128; }
+constexpr int tile_n(int t) { return t == k256x256 || t == kBig || t == k128x256 ? 256 : 128; }
 
 struct Plan {
   int tile, ksplit;
@@ -446,7 +628,7 @@ struct Plan {
 Plan plan_for(MxAct act, int m, int n, int k) {
   const int64_t t256 = (int64_t)((m + 255) / 256) * ((n + 255) / 256);
   const int stages = planes_of(act) * ((k + 127) / 128);
-  if (t256 >= 256 && act == kMxActFp4) return {k128x256, 1};
+  if (t256 >= 256 && act == kMxActFp4) return {kBig, 1};
   if (t256 >= 256) return {k128x128, 1};
   const int tile = m <= 64 ? k64x128 : k128x128;
   const int64_t tiles = (int64_t)((m + tile_m(tile) - 1) / tile_m(tile)) * ((n + tile_n(tile) - 1) / tile_n(tile));
@@ -455,9 +637,19 @@ Plan plan_for(MxAct act, int m, int n, int k) {
   return {tile, ks};
 }
 
+// Stages of 128 of K; in pairs for k256x256.
+int stages_of(const Plan &p, int k) { return p.tile == kBig ? (k + 255) / 256 * 2 : (k + 127) / 128; }
+
 template <int FA, bool TWO, class C>
 hipError_t tile_launch(const TileArgs &g, int tile, hipStream_t s) {
   const dim3 grid(g.tiles_m * g.tiles_n * g.ksplit);
+  if constexpr (FA == kMxFp4)
+    if (tile == kBig) {
+      const dim3 cus(std::min(g.tiles_m * g.tiles_n, 256));  // one workgroup per CU
+      if (g.bias) hipLaunchKernelGGL((k_mx_gemm_big<C, true>), cus, dim3(256), 0, s, g);
+      else hipLaunchKernelGGL((k_mx_gemm_big<C, false>), cus, dim3(256), 0, s, g);
+      return hipGetLastError();
+    }
   auto kern = tile == k256x256   ? k_mx_gemm_tile<FA, TWO, 2, 4, 8, 4, C>
               : tile == k128x256 ? k_mx_gemm_tile<FA, TWO, 2, 2, 8, 4, C>
               : tile == k128x128 ? k_mx_gemm_tile<FA, TWO, 2, 2, 4, 4, C>
@@ -470,8 +662,8 @@ hipError_t tile_launch(const TileArgs &g, int tile, hipStream_t s) {
 
 size_t mx_gemm_workspace_bytes(MxAct act, int m, int n, int k) {
   if (mx_rows_ok(act, m, n, k)) return mx_rows_workspace_bytes(act, m, n, k);
-  const int nk = (k + 127) / 128;
   const Plan p = plan_for(act, m, n, k);
+  const int nk = stages_of(p, k);
   return (digits(act) ? r256((size_t)planes_of(act) * m * k) : 0) + r256(packed_bytes(m, nk)) + r256(packed_bytes(n, nk)) +
          (p.ksplit > 1 ? (size_t)p.ksplit * m * n * 4 : 0);
 }
@@ -479,8 +671,8 @@ size_t mx_gemm_workspace_bytes(MxAct act, int m, int n, int k) {
 hipError_t launch_mx_gemm(MxAct act, const void *a, const void *w, const float *bias, void *c, bool c_bf16, int m,
                           int n, int k, void *ws, hipStream_t s) {
   if (mx_rows_ok(act, m, n, k)) return launch_mx_rows(act, a, w, bias, c, c_bf16, m, n, k, ws, s);
-  const int nk = (k + 127) / 128;
   const Plan plan = plan_for(act, m, n, k);
+  const int nk = stages_of(plan, k);
   const size_t mk = (size_t)m * k;
   uint8_t *p = static_cast<uint8_t *>(ws);
   uint8_t *planes = p;

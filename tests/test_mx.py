@@ -510,6 +510,16 @@ def test_product_matches_float64(rt, dev, act, m, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act,m,n,k,out", [(FP4, 4090, 4100, 32, "f32"), (FP4, 4096, 4104, 256, "bf16"), (FP4, 4000, 4097, 288, "bf16"),
+                                           (FP4, 4001, 4352, 640, "f32"), (FP4, 3841, 4088, 1056, "bf16"), (FP8, 4090, 4100, 160, "bf16"),
+                                           (FP8, 3900, 4097, 544, "f32"), ("f32", 3841, 4100, 96, "f32"), ("bf16", 4000, 4096, 416, "f32")])
+def test_products_of_many_tiles(rt, dev, act, m, n, k, out):
+    """Sizes that fill every CU with whole tiles, their last rows, columns and pieces of K ragged."""
+    a, w, a64, w64 = make(dev, act, m, n, k, 21)
+    check(product(rt, dev, act, a, w, m, n, k, out=out), a64, w64, act, k, out=out)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 6, 40, 200])
 def test_f32_activations_keep_their_bits(rt, dev, m):
     """Activations over 2^+-12 within a block, and rows at 2^90 and 2^-90, against the exact product."""
