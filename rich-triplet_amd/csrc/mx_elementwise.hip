@@ -56,16 +56,35 @@ __global__ __launch_bounds__(kThreads) void k_mx_dequantize(const uint8_t *__res
   }
 }
 
+template <int CTRL, int ROW_MASK = 0xF>
+RT_DEV double dpp_f64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = dpp_u32<CTRL, ROW_MASK>((uint32_t)b), hi = dpp_u32<CTRL, ROW_MASK>((uint32_t)(b >> 32));
+  return __builtin_bit_cast(double, (uint64_t)lo | (uint64_t)hi << 32);
+}
+
 // Sum of one double per thread over a workgroup of whole waves; `red` is a
 // fresh array of 16 for each call.
 RT_DEV double block_sum_f64(double v, double *red) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  v += dpp_f64<0xB1>(v);  // quad_perm [1,0,3,2]
+  v += dpp_f64<0x4E>(v);  // quad_perm [2,3,0,1]
+  v += dpp_f64<0x141>(v);  // row_half_mirror
+  v += dpp_f64<0x140>(v);  // row_mirror
+  v += dpp_f64<0x142, 0xA>(v);  // row_bcast15 into rows 1 and 3
+  v += dpp_f64<0x143, 0xC>(v);  // row_bcast31 into rows 2 and 3: lane 63 has the wave's sum
+  if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
   __syncthreads();
   double s = 0.0;
   for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += red[i];
   return s;
+}
+
+// 1 / sqrt(x): the instruction's 2^-26 or so and two Newton steps; 0 for infinity.
+RT_DEV double inv_sqrt(double x) {
+  double r = __builtin_amdgcn_rsq(x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) r *= __builtin_fma(-0.5 * x * r, r, 1.5);
+  return x == __builtin_inf() ? 0.0 : r;
 }
 
 // y as the f32 next to it that is odd in its last place, unless y is an f32: a
@@ -85,7 +104,7 @@ RT_DEV float f32_odd(double y) {
 template <int FMT, class T, int G>
 __global__ __launch_bounds__(1024) void k_add_rmsnorm_mx(const T *x, const float *residual,
                                                          const float *__restrict__ post,
-                                                         const float *__restrict__ gamma, double eps,
+                                                         const float *__restrict__ gamma, double eps, double inv_k,
                                                          uint8_t *__restrict__ elems, uint8_t *__restrict__ scales,
                                                          float *sum_out, int k, size_t row0) {
   __shared__ double red[2][16];
@@ -105,7 +124,7 @@ __global__ __launch_bounds__(1024) void k_add_rmsnorm_mx(const T *x, const float
     }
   }
   if (post) {
-    const double r = 1.0 / __builtin_sqrt(block_sum_f64(ss, red[0]) / k + eps);
+    const double r = inv_sqrt(block_sum_f64(ss, red[0]) * inv_k + eps);
 #pragma unroll
     for (int j = 0; j < G; ++j) {
       const int c = (int)threadIdx.x + j * (int)blockDim.x;
@@ -129,7 +148,7 @@ __global__ __launch_bounds__(1024) void k_add_rmsnorm_mx(const T *x, const float
       }
     }
   }
-  const double r = 1.0 / __builtin_sqrt(block_sum_f64(ss, red[1]) / k + eps);
+  const double r = inv_sqrt(block_sum_f64(ss, red[1]) * inv_k + eps);
 #pragma unroll
   for (int j = 0; j < G; ++j) {
     const int c = (int)threadIdx.x + j * (int)blockDim.x;
@@ -190,7 +209,7 @@ void norm_launch(const T *x, const float *residual, const float *post, const flo
   constexpr size_t kRowsPerLaunch = 1 << 21;  // a grid's threads stay below 2^32
   for (size_t r0 = 0; r0 < rows; r0 += kRowsPerLaunch)
     hipLaunchKernelGGL(kern, dim3((unsigned)std::min(rows - r0, kRowsPerLaunch)), block, 0, s, x, residual, post, gamma,
-                       (double)eps, elems, scales, sum_out, k, r0);
+                       (double)eps, 1.0 / k, elems, scales, sum_out, k, r0);
 }
 
 }  // namespace
