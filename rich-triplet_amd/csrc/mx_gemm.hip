@@ -136,7 +136,7 @@ struct TileArgs {
   size_t plane;            // bytes of one digit plane
   const float *bias;
   void *c;      // the result, or (ksplit > 1) the f32 partials [ksplit][M][N]
-  int M, N, K, nk, planes, tiles_m, tiles_n, ksplit;
+  int M, N, K, nk, tiles_m, tiles_n, ksplit;
   bool vec;  // rows of c are whole aligned 16-byte pieces
 };
 
@@ -188,24 +188,27 @@ RT_DEV void store_tile(const v4f (&acc)[NT][MT], uint8_t *stage, C *c, const flo
   }
 }
 
-// C tile of 16 NT WN columns (n) by 16 MT WM rows (m) by WN x WM waves, K in
-// stages of 128 through three LDS slots.  While the fragments of stage u are
-// multiplied, those of u+1 are read into the wave's other set of registers and
-// the copies of u+2 and u+3 are on their way; one barrier per stage.
+// C tile of 16 NT WN columns (n) by 16 MT WM rows (m) by WN x WM waves, in stages
+// of 128 of K and one of the P digit planes (p fastest: a weight's stage is copied
+// and read once for all planes), through three LDS slots each for the weight
+// (with both operands' scales) and the activations.  While the fragments of
+// stage u are multiplied, those of u+1 are read into the wave's other set of
+// registers and the copies of u+2 and u+3 are on their way; one barrier per stage.
 //
 // A slot row is a row's 64 (e2m1) or 128 (e4m3) bytes of the stage, in 16-byte
 // units; unit u of row r lies at u ^ (r / 2 % 4) or u ^ (r / 2 % 8): the rows that
 // a fragment read takes at once then lie on different banks (r / 4 % 4 took
-// twice the cycles per read).  Past the end of K the
-// copies read out of their buffer's range, which leaves zeros in LDS.
-template <int FA, bool TWO, int WN, int WM, int NT, int MT, class C>
+// twice the cycles per read).  Past the end of K the copies read out of their
+// buffer's range, which leaves zeros in LDS.
+template <int FA, bool TWO, int P, int WN, int WM, int NT, int MT, class C>
 __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
   constexpr int kWaves = WN * WM, BN = 16 * NT * WN, BM = 16 * MT * WM;
   constexpr int kARow = FA == kMxFp8 ? 128 : 64, kWBytes = BN * 64, kABytes = BM * kARow;
-  constexpr int kWScale = kWBytes + kABytes, kAScale = kWScale + 512 * ((BN + 127) / 128), kSlot = kAScale + 512 * ((BM + 127) / 128);
+  constexpr int kAScale = kWBytes + 512 * ((BN + 127) / 128), kWSlot = kAScale + 512 * ((BM + 127) / 128);
   constexpr int kWCopies = kWBytes / 1024 / kWaves, kACopies = kABytes / 1024 / kWaves;
   static_assert(kWBytes % (1024 * kWaves) == 0 && kABytes % (1024 * kWaves) == 0, "whole copies per wave");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[3 * kSlot];
+  constexpr int kALds = 3 * kWSlot, kLds = kALds + 3 * kABytes;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
   const int tid = (int)threadIdx.x, lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
   // XCD b % 8 gets a contiguous run of the (split, tile) items, tiles walked in
@@ -218,8 +221,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
   const int group = tile / (8 * g.tiles_n), in_group = tile % (8 * g.tiles_n), gm = min(8, g.tiles_m - group * 8);
   const int tm = group * 8 + in_group % gm, tn = in_group / gm;
   const int m0 = tm * BM, n0 = tn * BN, kb = g.K / 32;
-  const int total = g.planes * g.nk;
-  const int u0 = (int)((int64_t)split * total / g.ksplit), u1 = (int)((int64_t)(split + 1) * total / g.ksplit);
+  const int j0 = (int)((int64_t)split * g.nk / g.ksplit), j1 = (int)((int64_t)(split + 1) * g.nk / g.ksplit);
 
   // Copies: this lane's byte offsets from the tile's first row, and its unit's
   // block within a stage (to tell where the row ends).
@@ -253,35 +255,38 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
     const int blk = min((row0 >> 7) + (tile_rows == 256 ? sh : 0), last);
     return s + ((size_t)blk * g.nk + j) * 512 + 16 * sl;
   };
-  // The stage to copy next, u = j planes + p: a weight's stage serves all planes in turn.
-  int nj = u0 / g.planes, np = u0 - nj * g.planes, cp = np;
-  auto issue = [&](int slot) __attribute__((always_inline)) {
-    const int j = nj, p = np;
-    if (++np == g.planes) np = 0, ++nj;
-    uint8_t *base = lds + slot * kSlot;
-    if (wave == 0 && (BN == 256 || lane < 32))
-      __builtin_amdgcn_global_load_lds((gvoid *)scale_src(g.ws, n0, g.N, BN, j), (lvoid *)(base + kWScale), 16, 0, 0);
-    if (wave == 1 && (BM == 256 || lane < 32))
-      __builtin_amdgcn_global_load_lds((gvoid *)scale_src(g.as, m0, g.M, BM, j), (lvoid *)(base + kAScale), 16, 0, 0);
-    const uint8_t *ab = g.a + (size_t)p * g.plane + (size_t)m0 * arow;
-    const int left = kb - 4 * j;  // blocks of the row from this stage on
+  // Copies of the next stage, of plane p, into activation slot `slot`.
+  int jn = j0, wnext = 0;
+  auto issue = [&](auto pc, int slot) __attribute__((always_inline)) {
+    constexpr int p = decltype(pc)::value;
+    const int left = kb - 4 * jn;  // blocks of the row from this stage on
+    if constexpr (p == 0) {
+      uint8_t *base = lds + wnext * kWSlot;
+      if (wave == 0 && (BN == 256 || lane < 32))
+        __builtin_amdgcn_global_load_lds((gvoid *)scale_src(g.ws, n0, g.N, BN, jn), (lvoid *)(base + kWBytes), 16, 0, 0);
+      if (wave == 1 && (BM == 256 || lane < 32))
+        __builtin_amdgcn_global_load_lds((gvoid *)scale_src(g.as, m0, g.M, BM, jn), (lvoid *)(base + kAScale), 16, 0, 0);
 #pragma unroll
-    for (int i = 0; i < kWCopies; ++i)
-      copy_to_lds(wb, base + (kWCopies * wave + i) * 1024, wblk[i] < left ? (int)wo[i] : kOutOfRange, j * 64);
+      for (int i = 0; i < kWCopies; ++i)
+        copy_to_lds(wb, base + (kWCopies * wave + i) * 1024, wblk[i] < left ? (int)wo[i] : kOutOfRange, jn * 64);
+      wnext = wnext == 2 ? 0 : wnext + 1;
+    }
+    const uint8_t *ab = g.a + (size_t)p * g.plane + (size_t)m0 * arow;
 #pragma unroll
     for (int i = 0; i < kACopies; ++i)
-      copy_to_lds(ab, base + kWBytes + (kACopies * wave + i) * 1024, ablk[i] < left ? (int)ao[i] : kOutOfRange, j * kARow);
+      copy_to_lds(ab, lds + kALds + slot * kABytes + (kACopies * wave + i) * 1024, ablk[i] < left ? (int)ao[i] : kOutOfRange, jn * kARow);
+    if constexpr (p == P - 1) ++jn;
   };
 
   // Fragments: row l16 of tile i is 16 rows further per tile, whole swizzle periods.
   const uint32_t lb = lds_addr(lds);
   const uint32_t fw = lb + (16 * NT * wn + l16) * 64 + 16 * (grp ^ ((l16 >> 1) & 3));
-  const uint32_t fa0 = lb + kWBytes + (16 * MT * wm + l16) * kARow +
+  const uint32_t fa0 = lb + kALds + (16 * MT * wm + l16) * kARow +
                        16 * (FA == kMxFp8 ? grp ^ ((l16 >> 1) & 7) : grp ^ ((l16 >> 1) & 3));
-  const uint32_t fa1 = lb + kWBytes + (16 * MT * wm + l16) * kARow + 16 * ((4 + grp) ^ ((l16 >> 1) & 7));
+  const uint32_t fa1 = lb + kALds + (16 * MT * wm + l16) * kARow + 16 * ((4 + grp) ^ ((l16 >> 1) & 7));
   // a lane's scale bytes: [128 rows][64 lanes][8 tiles]
-  const uint32_t fws = lb + kWScale + (NT * wn / 8) * 512 + lane * 8 + (NT * wn) % 8;
-  const uint32_t fas = lb + kAScale + (MT * wm / 8) * 512 + lane * 8 + (MT * wm) % 8;
+  const uint32_t fws = lb + kWBytes + (NT * wn / 8) * 512 + lane * 8 + (NT * wn) % 8;
+  const uint32_t fas = lb + kAScale + (MT * wm / 8) * 512 + lane * 8 + (MT * wm) % 8 + (BM == 64 ? (m0 >> 4) & 4 : 0);
 
   v4f acc[NT][MT];
 #pragma unroll
@@ -290,47 +295,49 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
     for (int j = 0; j < MT; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
 
   constexpr int kUnits = FA == kMxFp8 ? 2 : 1;
-  struct Frag {
-    u32x4 w[NT], a[MT][kUnits];
+  struct WFrag {
+    u32x4 w[NT];
     uint32_t sw[NT / 4], sa[(MT + 3) / 4];
   };
-  auto read = [&](Frag &f, int slot) __attribute__((always_inline)) {
-    const uint32_t so = (uint32_t)slot * kSlot;
+  struct AFrag {
+    u32x4 a[MT][kUnits];
+  };
+  auto read_w = [&](WFrag &f, int slot) __attribute__((always_inline)) {
+    const uint32_t so = (uint32_t)slot * kWSlot;
 #pragma unroll
     for (int i = 0; i < NT / 4; ++i) f.sw[i] = lds_b32(fws + so + 4 * i);
     if constexpr (MT == 2) f.sa[0] = lds_u16(fas + so);
     else
 #pragma unroll
       for (int i = 0; i < MT / 4; ++i) f.sa[i] = lds_b32(fas + so + 4 * i);
-    steps<MT>([&](auto jc) __attribute__((always_inline)) {
-      constexpr int j = decltype(jc)::value;
-      f.a[j][0] = lds_b128<j * 16 * kARow>(fa0 + so);
-      if constexpr (kUnits == 2) f.a[j][1] = lds_b128<j * 16 * kARow>(fa1 + so);
-    });
     steps<NT>([&](auto ic) __attribute__((always_inline)) {
       constexpr int i = decltype(ic)::value;
       f.w[i] = lds_b128<i * 1024>(fw + so);
     });
   };
-  auto done = [&](Frag &f) __attribute__((always_inline)) {
+  auto read_a = [&](AFrag &f, int slot) __attribute__((always_inline)) {
+    const uint32_t so = (uint32_t)slot * kABytes;
+    steps<MT>([&](auto jc) __attribute__((always_inline)) {
+      constexpr int j = decltype(jc)::value;
+      f.a[j][0] = lds_b128<j * 16 * kARow>(fa0 + so);
+      if constexpr (kUnits == 2) f.a[j][1] = lds_b128<j * 16 * kARow>(fa1 + so);
+    });
+  };
+  auto done_w = [&](WFrag &f) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NT / 4; ++i) lds_done(f.sw[i]);
 #pragma unroll
     for (int i = 0; i < (MT + 3) / 4; ++i) lds_done(f.sa[i]);
 #pragma unroll
     for (int i = 0; i < NT; ++i) lds_done(f.w[i]);
+  };
+  auto done_a = [&](AFrag &f) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < MT; ++j)
 #pragma unroll
       for (int t = 0; t < kUnits; ++t) lds_done(f.a[j][t]);
   };
-  auto multiply = [&](Frag &f) __attribute__((always_inline)) {
-    if (g.planes > 1) {
-      const uint32_t less = 0x01010101u * kPlaneShift * (uint32_t)cp;
-#pragma unroll
-      for (int i = 0; i < (MT + 3) / 4; ++i) f.sa[i] -= less;  // no borrow: a digit block's byte is at least 20
-      cp = cp + 1 == g.planes ? 0 : cp + 1;
-    }
+  auto multiply = [&](AFrag &f, WFrag &w) __attribute__((always_inline)) {
     steps<MT>([&](auto jc) __attribute__((always_inline)) {
       constexpr int j = decltype(jc)::value;
       v8i av = {(int)f.a[j][0][0], (int)f.a[j][0][1], (int)f.a[j][0][2], (int)f.a[j][0][3], 0, 0, 0, 0};
@@ -344,54 +351,76 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
       }
       steps<NT>([&](auto ic) __attribute__((always_inline)) {
         constexpr int i = decltype(ic)::value;
-        const v8i wv = {(int)f.w[i][0], (int)f.w[i][1], (int)f.w[i][2], (int)f.w[i][3], 0, 0, 0, 0};
+        const v8i wv = {(int)w.w[i][0], (int)w.w[i][1], (int)w.w[i][2], (int)w.w[i][3], 0, 0, 0, 0};
         if constexpr (TWO)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, up, acc[i][j], 4, 0, i & 3, (int)f.sw[i / 4],
-                                                                       j & 3, (int)f.sa[j / 4]);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, up, acc[i][j], 4, 0, i & 3, (int)w.sw[i / 4],
+                                                                       j & 3, (int)w.sa[j / 4]);
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, av, acc[i][j], 4, FA == kMxFp8 ? 0 : 4, i & 3,
-                                                                     (int)f.sw[i / 4], j & 3, (int)f.sa[j / 4]);
+                                                                     (int)w.sw[i / 4], j & 3, (int)w.sa[j / 4]);
       });
     });
   };
 
-  // Waits count this wave's copies of whole stages; waves 0 and 1 issue one more
-  // (scales), the first of its stage, so they wait for at least as much.
-  constexpr int kCopies = kWCopies + kACopies;
-  const int n = u1 - u0;
-  issue(0);
-  if (n > 1) issue(1);
-  if (n > 2) issue(2);
-  if (n > 2) wait_vmcnt<2 * kCopies>();
-  else if (n > 1) wait_vmcnt<kCopies>();
+  // Copies of this wave in a stage of plane p.  Waves 0 and 1 issue one more
+  // (scales), the first of its stage: what the waits below leave outstanding is
+  // at most the later stages' copies all the same.
+  auto copies = [](int p) constexpr { return kACopies + (p % P == 0 ? kWCopies : 0); };
+  const int n = (j1 - j0) * P;
+  issue(IntC<0>{}, 0);
+  if (n > 1) issue(IntC<1 % P>{}, 1);
+  if (n > 2) issue(IntC<2 % P>{}, 2);
+  if (n > 2) wait_vmcnt<copies(1) + copies(2)>();
+  else if (n > 1) wait_vmcnt<copies(1)>();
   else wait_vmcnt<0>();
   wg_barrier();
-  Frag f0, f1;
-  read(f0, 0);
-  int slot = 0;
-  auto stage = [&](Frag &cur, Frag &nxt, int u) __attribute__((always_inline)) {
-    done(cur);
+  WFrag w0, w1;
+  AFrag a0, a1;
+  read_w(w0, 0);
+  read_a(a0, 0);
+  int slot = 0, wslot_r = 0;
+  auto stage = [&](auto pc, AFrag &cur, AFrag &nxt, WFrag &w, WFrag &wn_, int u) __attribute__((always_inline)) {
+    constexpr int p = decltype(pc)::value;
+    if constexpr (p == 0) done_w(w);
+    else
+#pragma unroll
+      for (int i = 0; i < (MT + 3) / 4; ++i) w.sa[i] -= 0x01010101u * kPlaneShift;  // no borrow: a digit block's byte is at least 20
+    done_a(cur);
     if (u + 1 < n) {
-      if (u + 2 < n) wait_vmcnt<kCopies>();
+      if (u + 2 < n) wait_vmcnt<copies(p + 2)>();
       else wait_vmcnt<0>();
       // every wave has read stage u and has its copies of stage u+1
       wg_barrier();
-      if (u + 3 < n) issue(slot);
+      if (u + 3 < n) issue(IntC<(p + 3) % P>{}, slot);
       slot = slot == 2 ? 0 : slot + 1;
-      read(nxt, slot);
+      read_a(nxt, slot);
+      if constexpr ((p + 1) % P == 0) {
+        wslot_r = wslot_r == 2 ? 0 : wslot_r + 1;
+        read_w(wn_, wslot_r);
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
-    multiply(cur);
+    multiply(cur, w);
     __builtin_amdgcn_sched_barrier(0);
   };
-  for (int u = 0; u < n; u += 2) {
-    stage(f0, f1, u);
-    if (u + 1 < n) stage(f1, f0, u + 1);
+  static_assert(P & 1, "a stage's registers alternate over two weight stages");
+  for (int u = 0; u < n; u += 2 * P) {
+    steps<P>([&](auto pc) __attribute__((always_inline)) {
+      constexpr int p = decltype(pc)::value;
+      if constexpr (p & 1) stage(pc, a1, a0, w0, w1, u + p);
+      else stage(pc, a0, a1, w0, w1, u + p);
+    });
+    if (u + P < n)
+      steps<P>([&](auto pc) __attribute__((always_inline)) {
+        constexpr int p = decltype(pc)::value;
+        if constexpr (p & 1) stage(pc, a0, a1, w1, w0, u + P + p);
+        else stage(pc, a1, a0, w1, w0, u + P + p);
+      });
   }
 
   // A lane holds columns 4 grp .. + 3 of each 16, row l16.  16 rows at a time go
   // through this wave's part of LDS and leave as whole row pieces, 16 bytes per lane.
-  if (n > 0) wg_barrier();  // other waves' last reads
-  uint8_t *buf = lds + wave * (3 * kSlot / kWaves);
+  wg_barrier();  // other waves' last reads
+  uint8_t *buf = lds + wave * (kLds / kWaves);
   const int row0 = m0 + 16 * MT * wm, col0 = n0 + 16 * NT * wn;
   if (g.ksplit > 1)
     store_tile<float, false, 0, NT>(acc, buf, static_cast<float *>(g.c) + (size_t)split * g.M * g.N, nullptr, row0, col0, g.M, g.N, g.vec);
@@ -618,43 +647,41 @@ int planes_of(MxAct act) { return act == kMxActF32 ? kPlanesF32 : act == kMxActB
 bool digits(MxAct act) { return act == kMxActF32 || act == kMxActBf16; }
 
 // C tiles: rows (m) by columns (n).
-enum Tile { k64x128, k128x128, k256x256, k128x256, kBig };
-constexpr int tile_m(int t) { return t == k64x128 ? 64 : t == k256x256 || t == kBig ? 256 : 128; }
-constexpr int tile_n(int t) { return t == k256x256 || t == kBig || t == k128x256 ? 256 : 128; }
+enum Tile { k64x128, k128x128, k256x256 };
+constexpr int tile_m(int t) { return t == k64x128 ? 64 : t == k256x256 ? 256 : 128; }
+constexpr int tile_n(int t) { return t == k256x256 ? 256 : 128; }
 
 struct Plan {
   int tile, ksplit;
 };
+// The largest tile that gives every CU one.  Fewer than 256 tiles of 128 x 128:
+// 64 x 128, and K split to about 480 workgroups, which run two or three to a CU
+// (us, 64 x 128 against 128 x 128, each with its best split: 77 x 10240 x 2560 in
+// bf16 20.5 : 22.6, 300 x 2560 x 10240 in MXFP8 31.6 : 34.1, 512 x 2560 x 10240 in
+// f32 72.5 : 72.1).  MXFP4 activations at 4096 x 10240 x 2560: 256 x 256 68 us.
 Plan plan_for(MxAct act, int m, int n, int k) {
-  const int64_t t256 = (int64_t)((m + 255) / 256) * ((n + 255) / 256);
-  const int stages = planes_of(act) * ((k + 127) / 128);
-  if (t256 >= 256 && act == kMxActFp4) return {kBig, 1};
-  if (t256 >= 256) return {k128x128, 1};
-  const int tile = m <= 64 ? k64x128 : k128x128;
-  const int64_t tiles = (int64_t)((m + tile_m(tile) - 1) / tile_m(tile)) * ((n + tile_n(tile) - 1) / tile_n(tile));
-  int ks = (int)std::min<int64_t>(std::max<int64_t>(512 / tiles, 1), 32);
-  ks = std::min(ks, std::max(stages / 4, 1));
-  return {tile, ks};
+  auto tiles = [&](int t) { return (int64_t)((m + tile_m(t) - 1) / tile_m(t)) * ((n + tile_n(t) - 1) / tile_n(t)); };
+  if (act == kMxActFp4 && tiles(k256x256) >= 256) return {k256x256, 1};
+  if (m > 64 && tiles(k128x128) >= 256) return {k128x128, 1};
+  const int64_t ks = std::max<int64_t>(480 / tiles(k64x128), 1);
+  return {k64x128, (int)std::min<int64_t>(ks, (k + 127) / 128)};
 }
 
 // Stages of 128 of K; in pairs for k256x256.
-int stages_of(const Plan &p, int k) { return p.tile == kBig ? (k + 255) / 256 * 2 : (k + 127) / 128; }
+int stages_of(const Plan &p, int k) { return p.tile == k256x256 ? (k + 255) / 256 * 2 : (k + 127) / 128; }
 
-template <int FA, bool TWO, class C>
+template <int FA, bool TWO, int P, class C>
 hipError_t tile_launch(const TileArgs &g, int tile, hipStream_t s) {
   const dim3 grid(g.tiles_m * g.tiles_n * g.ksplit);
   if constexpr (FA == kMxFp4)
-    if (tile == kBig) {
+    if (tile == k256x256) {
       const dim3 cus(std::min(g.tiles_m * g.tiles_n, 256));  // one workgroup per CU
       if (g.bias) hipLaunchKernelGGL((k_mx_gemm_big<C, true>), cus, dim3(256), 0, s, g);
       else hipLaunchKernelGGL((k_mx_gemm_big<C, false>), cus, dim3(256), 0, s, g);
       return hipGetLastError();
     }
-  auto kern = tile == k256x256   ? k_mx_gemm_tile<FA, TWO, 2, 4, 8, 4, C>
-              : tile == k128x256 ? k_mx_gemm_tile<FA, TWO, 2, 2, 8, 4, C>
-              : tile == k128x128 ? k_mx_gemm_tile<FA, TWO, 2, 2, 4, 4, C>
-                                 : k_mx_gemm_tile<FA, TWO, 2, 2, 4, 2, C>;
-  hipLaunchKernelGGL(kern, grid, dim3(tile == k256x256 ? 512 : 256), 0, s, g);
+  auto kern = tile == k64x128 ? k_mx_gemm_tile<FA, TWO, P, 2, 2, 4, 2, C> : k_mx_gemm_tile<FA, TWO, P, 2, 2, 4, 4, C>;
+  hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, g);
   return hipGetLastError();
 }
 
@@ -697,12 +724,20 @@ hipError_t launch_mx_gemm(MxAct act, const void *a, const void *w, const float *
   const bool to_part = plan.ksplit > 1;
   void *out = to_part ? static_cast<void *>(part) : c;
   const bool out16 = !to_part && c_bf16;
-  const TileArgs g{digits(act) ? planes : ae, we, as, wsc, mk, to_part ? nullptr : bias, out, m, n, k, nk, planes_of(act),
+  const TileArgs g{digits(act) ? planes : ae, we, as, wsc, mk, to_part ? nullptr : bias, out, m, n, k, nk,
                    (m + tile_m(plan.tile) - 1) / tile_m(plan.tile), (n + tile_n(plan.tile) - 1) / tile_n(plan.tile), plan.ksplit,
                    n % (out16 ? 8 : 4) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0};
-  if (act == kMxActFp4) e = out16 ? tile_launch<kMxFp4, false, uint16_t>(g, plan.tile, s) : tile_launch<kMxFp4, false, float>(g, plan.tile, s);
-  else if (act == kMxActFp8 && !c_bf16) e = tile_launch<kMxFp8, true, float>(g, plan.tile, s);
-  else e = out16 ? tile_launch<kMxFp8, false, uint16_t>(g, plan.tile, s) : tile_launch<kMxFp8, false, float>(g, plan.tile, s);
+  switch (act) {
+    case kMxActF32: e = tile_launch<kMxFp8, false, kPlanesF32, float>(g, plan.tile, s); break;
+    case kMxActBf16: e = tile_launch<kMxFp8, false, kPlanesBf16, float>(g, plan.tile, s); break;
+    case kMxActFp8:
+      e = !c_bf16 ? tile_launch<kMxFp8, true, 1, float>(g, plan.tile, s)
+          : out16 ? tile_launch<kMxFp8, false, 1, uint16_t>(g, plan.tile, s)
+                  : tile_launch<kMxFp8, false, 1, float>(g, plan.tile, s);
+      break;
+    default:
+      e = out16 ? tile_launch<kMxFp4, false, 1, uint16_t>(g, plan.tile, s) : tile_launch<kMxFp4, false, 1, float>(g, plan.tile, s);
+  }
   if (e != hipSuccess || !to_part) return e;
   return c_bf16 ? sum_launch<uint16_t>(part, bias, c, m, n, plan.ksplit, s) : sum_launch<float>(part, bias, c, m, n, plan.ksplit, s);
 }
