@@ -590,6 +590,7 @@ __global__ __launch_bounds__(256, 1) void k_mx_gemm_big(TileArgs g) {
       slot ^= 1;
     }
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last results, before anything reads them
+    done(f0);  // the next tile's first fragments: the code below may move their registers
     uint8_t *stage = lds + 2 * kSlot + wave * kStage;
     int m0, n0;
     corner(tile, m0, n0);
