@@ -123,7 +123,7 @@ size_t rt_gemm_workspace_held(void *stream);
 #define RT_LINEAR_F32 3    /* f32 [rows][cols] */
 #define RT_LINEAR_Q6K 4    /* planar Q6_K (rt_q6k_repack) */
 #define RT_LINEAR_Q8_0 5   /* planar Q8_0 (rt_q8_0_repack) */
-#define RT_LINEAR_MXFP4 6  /* planar MXFP4 (rt_mx_quantize) */
+#define RT_LINEAR_MXFP4 8  /* planar MXFP4 (rt_mx_quantize) */
 
 /* ---------------------------------------------------------------------------
  * Q6_K and Q8_0 weights kept packed on the device.  No counterpart in the

@@ -29,7 +29,7 @@ LIB_PATH = pathlib.Path(os.environ["RT_HIP_LIB"]).resolve() if os.environ.get("R
 RT_OK, RT_EINVAL, RT_EHIP, RT_ENOMEM, RT_ESTATE = 0, 1, 2, 3, 4
 
 
-LINEAR_Q4K, LINEAR_BF16, LINEAR_F32, LINEAR_Q6K, LINEAR_Q8_0, LINEAR_MXFP4 = 1, 2, 3, 4, 5, 6  # RT_LINEAR_* (rt_hip.h)
+LINEAR_Q4K, LINEAR_BF16, LINEAR_F32, LINEAR_Q6K, LINEAR_Q8_0, LINEAR_MXFP4 = 1, 2, 3, 4, 5, 8  # RT_LINEAR_* (rt_hip.h)
 MX_FP4, MX_FP8 = 4, 8  # RT_MX_*
 TYPE_F32, TYPE_BF16 = 0, 1  # RT_TYPE_*
 

@@ -159,9 +159,9 @@ def test_products_refuse_before_launch(rt, ptr):
     calls = {
         "mx": lambda a=ptr, w=ptr, c=ptr, m=1, n=4, k=32: L.rt_mx_gemm(FP8, a, w, None, 0, c, m, n, k, None),
         "rows": lambda a=ptr, w=ptr, c=ptr, m=1, n=4, k=32: L.rt_mxfp4_gemm(0, a, w, c, m, n, k, None),
-        "linear": lambda a=ptr, w=ptr, c=ptr, m=1, n=4, k=32: L.rt_qlinear_forward(6, w, None, a, c, m, n, k, None),
-        "gemm": lambda a=ptr, w=ptr, c=ptr, m=1, n=4, k=32: L.rt_linear_gemm_f32(6, w, a, c, m, n, k, None),
-        "batch": lambda a=ptr, w=ptr, c=ptr, m=1, n=4, k=32: L.rt_linear_gemv_batch(6, w, a, c, m, n, k, None),
+        "linear": lambda a=ptr, w=ptr, c=ptr, m=1, n=4, k=32: L.rt_qlinear_forward(rt.LINEAR_MXFP4, w, None, a, c, m, n, k, None),
+        "gemm": lambda a=ptr, w=ptr, c=ptr, m=1, n=4, k=32: L.rt_linear_gemm_f32(rt.LINEAR_MXFP4, w, a, c, m, n, k, None),
+        "batch": lambda a=ptr, w=ptr, c=ptr, m=1, n=4, k=32: L.rt_linear_gemv_batch(rt.LINEAR_MXFP4, w, a, c, m, n, k, None),
         "gemv": lambda a=ptr, w=ptr, c=ptr, m=1, n=4, k=32: L.rt_mxfp4_gemv(w, a, c, n, k, None),
     }
     for name, f in calls.items():
@@ -182,6 +182,15 @@ def test_products_refuse_before_launch(rt, ptr):
     refused(rt, L.rt_mx_gemm(FP4, ptr, ptr, None, 0, ptr + 2, 1, 4, 32, None), "aligned")
     refused(rt, L.rt_mx_gemm(FP4, ptr, ptr, None, 1, ptr + 1, 1, 4, 32, None), "aligned")
     refused(rt, L.rt_mxfp4_gemm(4, ptr, ptr, ptr, 1, 4, 32, None), "type 4")
+
+
+@pytest.mark.parametrize("fmt", [0, 6, 7, 9])
+def test_numbers_beside_the_formats_are_refused(rt, ptr, fmt):
+    """A format number that names no format never reaches a kernel."""
+    L = rt.lib()
+    assert L.rt_linear_gemm_f32(fmt, ptr, ptr, ptr, 1, 16, 256, None) == rt.RT_EINVAL
+    assert L.rt_qlinear_forward(fmt, ptr, None, ptr, ptr, 1, 16, 256, None) == rt.RT_EINVAL
+    assert L.rt_linear_gemv_batch(fmt, ptr, ptr, ptr, 1, 16, 256, None) == rt.RT_EINVAL
 
 
 def test_python_types(rt):
