@@ -294,9 +294,10 @@ rt_status rt_q4k_gemv_batch(const void *w, const float *a, float *c, int64_t m, 
 /* The same batched GEMV for the other projection formats a decode layer can
  * hold: gemv_bf16_t_batch (metal_decode.rs:527-558) for RT_LINEAR_BF16, and
  * RT_LINEAR_Q6K / RT_LINEAR_Q8_0 kept packed (planar layout, rt_q6k_repack /
- * rt_q8_0_repack) where the reference widens them to BF16 first.  Reads the
+ * rt_q8_0_repack) where the reference widens them to BF16 first; also
+ * RT_LINEAR_MXFP4 (rt_mxfp4_gemm's arithmetic).  Reads the
  * weights once for all m = 1..8 rows; device pointers, a and w 16-byte
- * aligned; k % 256 == 0 for Q6_K, k % 64 == 0 otherwise; fmt RT_LINEAR_Q4K
+ * aligned; k % 256 == 0 for Q6_K, k % 32 == 0 for MXFP4, k % 64 == 0 otherwise; fmt RT_LINEAR_Q4K
  * is rt_q4k_gemv_batch.  Workspace as rt_q4k_gemv_batch. */
 rt_status rt_linear_gemv_batch(int32_t fmt, const void *w, const float *a, float *c, int64_t m, int64_t n, int64_t k,
                                void *stream);
@@ -364,11 +365,12 @@ rt_status rt_decode_destroy(rt_decode *d);
  * exponents of each Q4_K weight are computed here, once: 4 bytes per row). */
 rt_status rt_decode_set_layer(rt_decode *d, int32_t layer, const rt_gemma3_layer *w, int32_t device_ptrs);
 /* Same, with the format of each projection in the order q, k, v, o, gate,
- * up, down: RT_LINEAR_Q4K, RT_LINEAR_Q6K, RT_LINEAR_Q8_0 or RT_LINEAR_BF16
- * (the device layouts of rt_gguf_load_linear_ex).  The reference's context
+ * up, down: RT_LINEAR_Q4K, RT_LINEAR_Q6K, RT_LINEAR_Q8_0, RT_LINEAR_BF16 (the
+ * device layouts of rt_gguf_load_linear_ex) or RT_LINEAR_MXFP4 (rt_mx_quantize;
+ * input widths of whole 64).  The reference's context
  * takes Q4_K or BF16 per projection (upload_linear_detect_type,
  * metal_decode.rs:1259-1277, with Q6_K/Q8_0 widened to BF16 at load); here
- * Q6_K and Q8_0 also run natively, in decode, batch and prefill.
+ * Q6_K, Q8_0 and MXFP4 also run natively, in decode, batch and prefill.
  * Failure (a null or misaligned pointer, an unsupported format, a failed
  * upload) is checked before anything is uploaded, and the new binding
  * replaces the old one only when it is whole; but a failed call still
@@ -451,7 +453,7 @@ rt_status rt_decode_memory(const rt_decode *d, rt_decode_memory_info *out);
 /* How rt_decode_step_batch runs (no counterpart in the reference, whose
  * verify batch always runs its batched GEMVs): *batched = 1 when every bound
  * layer's projections are served by the batched GEMVs (Q4_K, Q6_K, Q8_0,
- * BF16) and the M tokens go through each layer together, reading each
+ * BF16, MXFP4) and the M tokens go through each layer together, reading each
  * weight once; 0 when they run as M single-token passes. */
 rt_status rt_decode_verify_batched(const rt_decode *d, int32_t *batched);
 /* Device buffers of the context, for inspection. */

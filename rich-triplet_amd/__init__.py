@@ -330,13 +330,15 @@ def q4k_gemv_multi(ws, ys, ns, x, k: int, stream=None) -> None:
 
 def linear_gemm_f32(fmt: int, w, a, c, m: int, n: int, k: int, stream=None) -> None:
     """c[m][n] = a[m][k] . W[n][k] for a weight in format fmt (LINEAR_Q4K,
-    LINEAR_BF16, LINEAR_Q6K or LINEAR_Q8_0, the last two planar)."""
+    LINEAR_BF16, LINEAR_F32, LINEAR_Q6K, LINEAR_Q8_0 or LINEAR_MXFP4, the last
+    three planar)."""
     check(lib().rt_linear_gemm_f32(fmt, _p(w), _p(a), _p(c), m, n, k, _stream(stream)))
 
 
 def qlinear_forward(fmt: int, w, x, out, m: int, n: int, k: int, bias=None, stream=None) -> None:
     """QLinear::forward: out[m][n] = x[m][k] . W[n][k] (+ bias[n]) for a weight of
-    format fmt (LINEAR_Q4K, LINEAR_BF16, LINEAR_F32, LINEAR_Q6K or LINEAR_Q8_0)."""
+    format fmt (LINEAR_Q4K, LINEAR_BF16, LINEAR_F32, LINEAR_Q6K, LINEAR_Q8_0 or
+    LINEAR_MXFP4)."""
     check(lib().rt_qlinear_forward(fmt, _p(w), None if bias is None else _p(bias), _p(x), _p(out), m, n, k,
                                    _stream(stream)))
 

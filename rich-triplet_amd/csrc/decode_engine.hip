@@ -295,6 +295,7 @@ static size_t proj_bytes(int fmt, size_t rows, size_t cols) {
     case RT_LINEAR_Q6K: return cols % 256 ? 0 : rows * (cols / 256) * 210;
     case RT_LINEAR_Q8_0: return cols % 32 ? 0 : rows * (cols / 32) * 34;
     case RT_LINEAR_BF16: return cols % 8 ? 0 : rows * cols * 2;
+    case RT_LINEAR_MXFP4: return cols % 64 ? 0 : rows * (cols / 32) * 17;  // the prefill GEMM's stages are 64 wide
     default: return 0;
   }
 }
@@ -355,7 +356,7 @@ rt_status rt_decode_set_layer_formats(rt_decode *d, int32_t layer, const rt_gemm
     if (!d->fused && !rows_mb_formats_ok(d->shape, formats))
       return unset(set_error(RT_EINVAL,
                              "rt_decode_set_layer: this shape runs on the rows kernels, whose batched GEMVs take "
-                             "Q4_K, Q6_K (whole super-blocks), Q8_0 and BF16 projections"));
+                             "Q4_K, Q6_K (whole super-blocks), Q8_0, BF16 and MXFP4 projections"));
   }
   // Every pointer is checked before anything is freed or uploaded; the new
   // binding is built aside and replaces the old one only when it is whole.

@@ -24,6 +24,7 @@
 #include "q4k_gemv.hpp"
 #include "q4k_gemv_mb.hpp"
 #include "kquant_tile.hpp"
+#include "mx_kernels.hpp"
 #include "rt_device.hpp"
 #include "rt_kernels.hpp"
 #include "rt_capi_util.hpp"
@@ -1082,6 +1083,7 @@ static void launch_proj(Launch &l, int fmt, const uint8_t *W, const float *x, fl
     case RT_LINEAR_Q6K: l.err = launch_q6k_gemv(W, x, y, n, k, l.s); break;
     case RT_LINEAR_Q8_0: l.err = launch_q8_0_gemv(W, x, y, n, k, l.s); break;
     case RT_LINEAR_BF16: l.err = launch_bf16_gemv(reinterpret_cast<const uint16_t *>(W), x, y, n, k, l.s); break;
+    case RT_LINEAR_MXFP4: l.err = launch_mx_gemv(W, x, y, n, k, l.s); break;
     default: l.err = launch_q4k_gemv(W, x, y, n, k, l.s); break;
   }
 }

@@ -39,6 +39,7 @@
 #include "gemma3_math.hpp"
 #include "kquant_layout.hpp"
 #include "q4k_gemv.hpp"
+#include "mx_kernels.hpp"
 #include "rt_device.hpp"
 #include "rt_kernels.hpp"
 
@@ -773,6 +774,7 @@ static hipError_t any_proj(int fmt, const uint8_t *W, const float *x, float *y, 
     case RT_LINEAR_Q6K: return launch_q6k_gemv(W, x, y, n, k, s);
     case RT_LINEAR_Q8_0: return launch_q8_0_gemv(W, x, y, n, k, s);
     case RT_LINEAR_BF16: return launch_bf16_gemv(reinterpret_cast<const uint16_t *>(W), x, y, n, k, s);
+    case RT_LINEAR_MXFP4: return launch_mx_gemv(W, x, y, n, k, s);
     default: return launch_q4k_gemv(W, x, y, n, k, s);
   }
 }

@@ -28,7 +28,12 @@ hipError_t launch_mx_gemm(MxAct act, const void *a, const void *w, const float *
 // The same for few rows (mx_rows.hip), which launch_mx_gemm takes where it serves.
 bool mx_rows_ok(MxAct act, int m, int n, int k);
 size_t mx_rows_workspace_bytes(MxAct act, int m, int n, int k);
+// split_done: ws holds this a's digit columns already, from a call with the same act, a, m and k.
 hipError_t launch_mx_rows(MxAct act, const void *a, const void *w, const float *bias, void *c, bool c_bf16, int m,
-                          int n, int k, void *ws, hipStream_t s);
+                          int n, int k, void *ws, hipStream_t s, bool split_done = false);
+// y = W x of one f32 row; no workspace.
+inline hipError_t launch_mx_gemv(const void *w, const float *x, float *y, int n, int k, hipStream_t s) {
+  return launch_mx_rows(kMxActF32, x, w, nullptr, y, false, 1, n, k, nullptr, s);
+}
 
 }  // namespace rt

@@ -267,7 +267,7 @@ size_t mx_rows_workspace_bytes(MxAct act, int m, int n, int k) {
 }
 
 hipError_t launch_mx_rows(MxAct act, const void *a, const void *w, const float *bias, void *c, bool c_bf16, int m,
-                          int n, int k, void *ws, hipStream_t s) {
+                          int n, int k, void *ws, hipStream_t s, bool split_done) {
   const RowsPlan p = rows_plan(act, m, n, k);
   const int nmac = (k + kMacro - 1) / kMacro;
   const uint8_t *we = static_cast<const uint8_t *>(w), *ae = static_cast<const uint8_t *>(a);
@@ -275,7 +275,8 @@ hipError_t launch_mx_rows(MxAct act, const void *a, const void *w, const float *
   if (p.split) {
     uint8_t *cols = static_cast<uint8_t *>(ws), *sc = cols + r256((size_t)nmac * p.ct * 8192);
     const dim3 grid((unsigned)(((int64_t)m * nmac * (kMacro / 8) + 255) / 256)), block(256);
-    if (act == kMxActF32)
+    if (split_done) {
+    } else if (act == kMxActF32)
       hipLaunchKernelGGL((k_mx_split_cols<float, kPlanesF32>), grid, block, 0, s, static_cast<const float *>(a), cols, sc, m, k, nmac, p.ct);
     else
       hipLaunchKernelGGL((k_mx_split_cols<uint16_t, kPlanesBf16>), grid, block, 0, s, static_cast<const uint16_t *>(a), cols, sc, m, k, nmac, p.ct);

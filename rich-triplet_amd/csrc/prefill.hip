@@ -26,6 +26,7 @@
 #include "decode.hpp"
 #include "gemma3_math.hpp"
 #include "q4k_gemv_mb.hpp"
+#include "mx_kernels.hpp"
 #include "rt_device.hpp"
 #include "rt_kernels.hpp"
 
@@ -790,14 +791,18 @@ size_t rows_mb_part_bytes(const DecodeShape &s) {
   auto set = [](int n, int k) {
     return std::max(k % 256 == 0 ? mb_part_bytes(n, k) : (size_t)0, kquant_mb_part_bytes(n, k));
   };
-  return std::max({set(QD + 2 * KVD, H), set(H, QD), set(2 * F, H), set(H, F)});
+  // the digit columns of a set's MXFP4 matrices come after them
+  auto mx = [](int n, int k) { return mx_rows_workspace_bytes(kMxActF32, kMaxBatch, n, k); };
+  return std::max({set(QD + 2 * KVD, H), set(H, QD), set(2 * F, H), set(H, F)}) + std::max({mx(F, H), mx(H, QD), mx(H, F)});
 }
 
 bool rows_mb_formats_ok(const DecodeShape &s, const int *fmt) {
   const int H = s.hidden, F = s.ffn, QD = s.n_q_heads * s.head_dim;
   const int kdim[7] = {H, H, H, QD, H, H, F};
   for (int i = 0; i < 7; ++i) {
-    const bool ok = fmt[i] == RT_LINEAR_Q4K ? kdim[i] % 256 == 0 : kquant_mb_supported(fmt[i], kdim[i]);
+    const bool ok = fmt[i] == RT_LINEAR_Q4K    ? kdim[i] % 256 == 0
+                    : fmt[i] == RT_LINEAR_MXFP4 ? kdim[i] % 64 == 0
+                                                : kquant_mb_supported(fmt[i], kdim[i]);
     if (!ok) return false;
   }
   return true;
@@ -859,6 +864,18 @@ hipError_t enqueue_rows(const DecodeShape &s, const DecodeArgs &a, const LayerAr
         if (r != hipSuccess) return r;
         for (int c = 0; c < cnt; ++c) *gv[c] = out[c];
         part += (fmt == RT_LINEAR_Q4K ? mb_part_bytes(ntot, K) : kquant_mb_part_bytes(ntot, K)) / sizeof(float);
+      }
+      // MXFP4 matrices: from the f32 rows, split into digits once for the set
+      int i = 0;
+      bool split = false;
+      for (const MbMat &m : mats) {
+        if (fmts.begin()[i] == RT_LINEAR_MXFP4) {
+          hipError_t r = launch_mx_rows(kMxActF32, A, m.w, nullptr, m.y, false, n, m.n, K, part, st, split);
+          if (r != hipSuccess) return r;
+          split = true;
+          *views.begin()[i] = rows_plain(m.y, m.n);
+        }
+        ++i;
       }
       return hipSuccess;
     }

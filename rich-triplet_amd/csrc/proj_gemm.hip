@@ -18,6 +18,7 @@
 #include "../../include/rt_hip.h"
 #include "kquant_layout.hpp"
 #include "mfma_common.hpp"
+#include "mx_common.hpp"
 #include "rt_device.hpp"
 #include "rt_kernels.hpp"
 
@@ -43,6 +44,13 @@ RT_DEV void proj_load8(const uint8_t *__restrict__ W, int N, int K, int n, int p
     const uint32_t u[2] = {q.x, q.y};
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = d * (float)(int8_t)(u[i >> 2] >> (8 * (i & 3)));
+  } else if constexpr (FMT == RT_LINEAR_MXFP4) {
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    const uint32_t q = reinterpret_cast<const uint32_t *>(W)[(size_t)n * (K / 8) + p];
+    const float s = mx_scale(W[(size_t)N * K / 2 + (size_t)n * (K / 32) + (p >> 2)]);
+    const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 1);
+    const v2f c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 3);
+    v[0] = a.x * s, v[1] = a.y * s, v[2] = b.x * s, v[3] = b.y * s, v[4] = c.x * s, v[5] = c.y * s, v[6] = d.x * s, v[7] = d.y * s;
   } else if constexpr (FMT == RT_LINEAR_Q4K) {
     const uint8_t *blk = W + ((size_t)n * (K / 256) + (p >> 5)) * kQ4KBlockBytes;
     const int c = (p >> 3) & 3, h = (p >> 2) & 1;  // chunk, its low or high nibbles
@@ -598,6 +606,7 @@ static hipError_t proj_gemm(const void *a, bool a_bf16, int am, _Float16 *a16, i
     case RT_LINEAR_Q8_0: RT_WIDEN(RT_LINEAR_Q8_0, RT_LINEAR_F32); break;
     case RT_LINEAR_BF16: RT_WIDEN(RT_LINEAR_BF16, RT_LINEAR_F32); break;
     case RT_LINEAR_F32: RT_WIDEN(RT_LINEAR_F32, RT_LINEAR_F32); break;
+    case RT_LINEAR_MXFP4: RT_WIDEN(RT_LINEAR_MXFP4, RT_LINEAR_F32); break;
     default: return hipErrorInvalidValue;
   }
 #undef RT_WIDEN

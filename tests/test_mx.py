@@ -12,6 +12,8 @@ import math
 import numpy as np
 import pytest
 
+from conftest import rel_l2
+
 FP4, FP8 = 4, 8
 EMAX, TOP = {FP4: 2, FP8: 8}, {FP4: 6.0, FP8: 448.0}
 E2M1 = np.array([0, .5, 1, 1.5, 2, 3, 4, 6], np.float64)
@@ -729,3 +731,115 @@ def test_capture_that_would_allocate_is_refused(rt, dev):
     s.synchronize()
     assert bool((c == 0).all()) and rt.gemm_workspace_held(s) > 0
     rt.gemm_workspace_release(s)
+
+
+# --- the decode engine with MXFP4 projections -------------------------------
+PROJ = ("q", "k", "v", "o", "gate", "up", "down")
+MX, Q8_0, BF16, Q6K = 8, 5, 2, 4
+ENGINE = {  # layer -> projection -> format, Q4_K otherwise
+    # every set by itself, behind Q4_K sets, and beside each other format
+    "tiny": {0: {p: MX for p in PROJ}, 1: dict(v=MX, down=MX), 2: dict(q=MX, up=MX), 3: dict(q=Q8_0, k=MX, v=BF16, o=MX),
+             4: dict(q=MX, k=Q6K, v=MX, gate=Q8_0, up=MX), 5: {p: MX for p in PROJ}},
+    "768": {0: {p: MX for p in PROJ}, 1: dict(v=MX, gate=MX, down=MX), 2: dict(q=MX, k=Q8_0, v=MX, o=MX, up=MX)},
+    "1152": {0: dict({p: Q8_0 for p in PROJ}, v=MX, o=MX, down=MX), 1: {p: MX for p in PROJ}},
+}
+
+
+def engine_cfg(shape):
+    if shape == "tiny":
+        from test_gpu_decode import tiny
+        return tiny(2)
+    hidden, ffn, heads, dim = dict(zip(("768", "1152"), ((768, 1536, 4, 128), (1152, 6912, 4, 256))))[shape]
+    return dict(hidden=hidden, ffn=ffn, n_q_heads=heads, n_kv_heads=1, head_dim=dim, n_layers=len(ENGINE[shape]), vocab=777,
+                sliding_window=9, global_every=2, rope_theta_local=10000.0, rope_theta_global=1000000.0,
+                rope_fs_local=1.0, rope_fs_global=0.125, eps=1e-6, attn_scale=1.0 / math.sqrt(dim))
+
+
+def engine_model(orc, shape, max_seq, ctx, seed):
+    """The oracle's layers hold an MXFP4 projection's values as bf16, which has
+    every one of them (2 significant bits); the device's hold its bytes."""
+    from test_kquant import SHAPES, apply_formats
+    from test_oracle import make_model
+    cfg, plan = engine_cfg(shape), ENGINE[shape]
+    if cfg["hidden"] % 256:  # no Q4_K blocks: make_model's weights are replaced by the plan's, which has every projection
+        layers, embed, fnorm = make_model_any(orc, cfg, max_seq, ctx, seed)
+    else:
+        layers, embed, fnorm = make_model(orc, cfg, max_seq=max_seq, ctx=ctx, seed=seed)
+    as_bf16 = {li: {p: BF16 if f == MX else f for p, f in d.items()} for li, d in plan.items()}
+    dev_layers, fmts = apply_formats(orc, cfg, layers, as_bf16, seed=seed + 1)
+    for li, d in plan.items():
+        for p, f in d.items():
+            if f != MX:
+                continue
+            x = (layers[li][p].astype(np.uint32) << 16).view(np.float32).astype(np.float64).reshape(SHAPES(cfg)[p])
+            dev_layers[li][p] = planar(x, FP4)
+            v = values(x, FP4).astype(np.float32).reshape(-1)
+            layers[li][p] = (v.view(np.uint32) >> 16).astype(np.uint16)
+            assert np.array_equal((layers[li][p].astype(np.uint32) << 16).view(np.float32), v)
+            fmts[li][PROJ.index(p)] = MX
+    return cfg, layers, dev_layers, fmts, embed, fnorm
+
+
+def make_model_any(orc, cfg, max_seq, ctx, seed):
+    rng = np.random.default_rng(seed)
+    H, D, KVD = cfg["hidden"], cfg["head_dim"], cfg["n_kv_heads"] * cfg["head_dim"]
+    layers = []
+    for _ in range(cfg["n_layers"]):
+        L = {n: (0.1 * rng.normal(size=s)).astype(np.float32) for n, s in
+             dict(in_norm=H, post_attn_norm=H, pre_ffn_norm=H, post_ffn_norm=H, q_norm=D, k_norm=D).items()}
+        for c in ("k_cache", "v_cache"):
+            L[c] = np.zeros((max_seq, KVD), np.float32)
+            L[c][:ctx] = rng.normal(size=(ctx, KVD))
+        layers.append(L)
+    return layers, orc.synth_bf16(seed, cfg["vocab"] * H), (0.1 * rng.normal(size=H)).astype(np.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", ENGINE)
+def test_engine_steps_and_verify_batch(rt, orc, shape):
+    """Steps (one eager, the others replays), then batches of 3 and of 8, against
+    the oracle on the same values.  Tolerance: the engine's for every format."""
+    from test_kquant import mixed_ctx
+    ctx, max_seq = 6, 40
+    cfg, layers, dev_layers, fmts, embed, fnorm = engine_model(orc, shape, max_seq, ctx, 9000)
+    d = mixed_ctx(rt, cfg, dev_layers, fmts, embed, fnorm, ctx, max_seq, layers)
+    assert d.verify_batched
+    for tok in (11, 3, 700):
+        got = d.decode_step(tok, ctx)
+        ref = orc.gemma3_decode_step(cfg, layers, embed, fnorm, token=tok, pos=ctx)
+        print(f"step {ctx}: {rel_l2(got, ref):.2e}", flush=True)
+        assert rel_l2(got, ref) < 1e-3, (ctx, rel_l2(got, ref))
+        ctx += 1
+    for m in (3, 8):
+        toks = [(31 * i + m) % cfg["vocab"] for i in range(m)]
+        for _ in range(2):  # the second is a replay
+            got = d.decode_step_batch(toks, ctx)
+        for i, tok in enumerate(toks):
+            ref = orc.gemma3_decode_step(cfg, layers, embed, fnorm, token=tok, pos=ctx + i)
+            print(f"batch {m} row {i}: {rel_l2(got[i], ref):.2e}", flush=True)
+            assert rel_l2(got[i], ref) < 1e-3, (m, i, rel_l2(got[i], ref))
+        ctx += m
+    d.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,T,mode,chunk", [("tiny", 3, 1, 0), ("tiny", 20, 0, 0), ("768", 37, 1, 0), ("1152", 30, 1, 7)])
+def test_engine_prefill(rt, orc, shape, T, mode, chunk):
+    """Prompts through the GEMM on widened rows and, in chunks of 7, through the
+    batched products; the step after a prompt reads its cache."""
+    from test_kquant import plain_ctx
+    from test_prefill import LOGITS_TOL, fresh_caches
+    cfg, layers, dev_layers, fmts, embed, fnorm = engine_model(orc, shape, 48, 0, 9100 + T)
+    d = plain_ctx(rt, cfg, dev_layers, fmts, embed, fnorm, 48)
+    if chunk:
+        d.set_prefill_chunk(chunk)
+    toks = [(17 * i + 4) % cfg["vocab"] for i in range(T)]
+    got = d.prefill(toks, 0, mode)
+    ref_layers = fresh_caches(layers)
+    ref = orc.gemma3_prefill(cfg, ref_layers, embed, fnorm, toks, 0, mode)
+    print(f"prefill: {rel_l2(got, ref):.2e}", flush=True)
+    assert rel_l2(got, ref) < LOGITS_TOL, rel_l2(got, ref)
+    if mode == 1:
+        ref = orc.gemma3_decode_step(cfg, ref_layers, embed, fnorm, token=9, pos=T)
+        assert rel_l2(d.decode_step(9, T), ref) < LOGITS_TOL
+    d.close()
