@@ -195,7 +195,9 @@ rt_status rt_q8_0_gemv(const void *w, const float *x, float *y, int64_t n, int64
 /* Types of ordinary arrays in the calls below. */
 #define RT_TYPE_F32 0
 #define RT_TYPE_BF16 1
-/* Bytes of a microscaled [rows][k] tensor (0 for a bad format or k). */
+/* Bytes of a microscaled [rows][k] tensor (0 for a bad format, k or rows, and
+ * past the 2^48 elements that the calls below take).  In all of them no output
+ * overlaps an input, but where it is said. */
 size_t rt_mx_bytes(int32_t fmt, int64_t rows, int64_t k);
 /* Quantises x [rows][k] (RT_TYPE_*): a block's scale is the exponent of its
  * largest magnitude less the element type's (8 for e4m3, 2 for e2m1), elements
@@ -233,9 +235,10 @@ rt_status rt_gelu_mul_mx(int32_t type, const void *gate, const void *up, int64_t
  * (RT_MX_FP8 or RT_MX_FP4), W RT_LINEAR_MXFP4, c f32 or bf16 (c_type), on the
  * scaled matrix instructions with f32 accumulation: c carries the sum's
  * rounding alone, but that an MXFP8 product into bf16 may lose terms below
- * 2^-13 of the largest of their eight neighbours in k (5e-6 of c's norm).  k % 32 == 0; a and w 16-byte aligned.
- * Workspace of rt_q4k_gemm_f32: up to (m + n) * k / 32 bytes, plus split-K
- * partials. */
+ * 2^-13 of the largest of their eight neighbours in k (5e-6 of c's norm).
+ * k % 32 == 0, k <= 2^22, m <= 2^30, n <= 2^26; a and w 16-byte aligned.
+ * Workspace of rt_q4k_gemm_f32: up to (m + n) * k / 32 bytes (each rounded up to
+ * whole tiles), plus split-K partials. */
 rt_status rt_mx_gemm(int32_t a_fmt, const void *a, const void *w, const float *bias, int32_t c_type, void *c,
                      int64_t m, int64_t n, int64_t k, void *stream);
 /* c[m][n] = a[m][k] . W[n][k] with activations in f32 or bf16 (a_type) on an
@@ -267,7 +270,8 @@ rt_status rt_mxfp4_gemv(const void *w, const float *x, float *y, int64_t n, int6
  * (m + n) * k * 2 bytes (m * k * 2, in whole groups of 32 rows, for Q4_K, and
  * for Q6_K and Q8_0 of up to 384 rows, or up to 1024 where k <= 4096 and
  * m * n <= 2,600,000, which stay packed; none for the f32 GEMV), plus split-K
- * partials. */
+ * partials.  RT_LINEAR_MXFP4: rt_mxfp4_gemm, with its arithmetic, limits and
+ * workspace (k % 32 == 0). */
 rt_status rt_linear_gemm_f32(int32_t fmt, const void *w, const float *a, float *c, int64_t m, int64_t n, int64_t k,
                              void *stream);
 /* QLinear::forward (qlinear.rs:82-111): out[m][n] = x[m][k] . W[n][k], then

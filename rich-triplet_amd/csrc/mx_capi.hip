@@ -30,8 +30,9 @@ rt_status check_product(const char *who, const void *a, const void *w, const flo
     return set_error(RT_EINVAL, "%s: m=%lld n=%lld k=%lld must be positive", who, (long long)m, (long long)n, (long long)k);
   if (k % kMxBlock != 0) return set_error(RT_EINVAL, "%s: k=%lld must be a multiple of 32", who, (long long)k);
   if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return set_error(RT_EINVAL, "%s: m, n or k exceeds int32", who);
-  // 256 rows of either operand stay below 2^31 bytes, the tiles of c below 2^31
-  if (k > (1 << 22) || m > (int64_t(1) << 40) / n)
+  // 256 rows of either operand stay below 2^31 bytes, a grid's threads below 2^32
+  // (n of a token's product: 16 rows to a workgroup of up to 640)
+  if (k > (1 << 22) || m > (1 << 30) || n > (1 << 26) || m > (int64_t(1) << 38) / n)
     return set_error(RT_EINVAL, "%s: m=%lld n=%lld k=%lld is too large", who, (long long)m, (long long)n, (long long)k);
   if (!a || !w || !c) return set_error(RT_EINVAL, "%s: null pointer", who);
   if (!aligned16(a) || !aligned16(w)) return set_error(RT_EINVAL, "%s: a and w must be 16-byte aligned", who);
@@ -56,7 +57,9 @@ rt_status rt::mx_product(const char *who, int act, const void *a, const void *w,
 extern "C" {
 
 size_t rt_mx_bytes(int32_t fmt, int64_t rows, int64_t k) {
-  if ((fmt != RT_MX_FP4 && fmt != RT_MX_FP8) || rows <= 0 || k <= 0 || k % kMxBlock != 0) return 0;
+  if ((fmt != RT_MX_FP4 && fmt != RT_MX_FP8) || rows <= 0 || k <= 0 || k % kMxBlock != 0 || k > INT32_MAX ||
+      rows > (int64_t(1) << 48) / k)
+    return 0;
   const size_t n = (size_t)rows * (size_t)k;
   return mx_elem_bytes(fmt, n) + n / kMxBlock;
 }

@@ -99,6 +99,7 @@ def test_mx_bytes(rt):
     assert rt.mx_bytes(rt.MX_FP4, 3, 64) == 3 * 32 + 6
     assert rt.mx_bytes(rt.MX_FP4, 3, 65) == 0 and rt.mx_bytes(5, 3, 64) == 0 and rt.mx_bytes(rt.MX_FP8, 0, 64) == 0
     assert rt.mx_bytes(rt.MX_FP8, 1 << 27, 1 << 10) == (1 << 37) + (1 << 32)
+    assert rt.mx_bytes(rt.MX_FP8, 1 << 62, 1 << 10) == 0
 
 
 def test_conversions_refuse_before_launch(rt, ptr):
@@ -171,6 +172,8 @@ def test_products_refuse_before_launch(rt, ptr):
         refused(rt, f(n=0), "positive")
         refused(rt, f(k=-32), "positive")
         refused(rt, f(n=1 << 31), "int32")
+        refused(rt, f(n=1 << 27), "too large")  # a grid's threads pass 2^32
+        refused(rt, f(k=1 << 23), "too large")
         for arg in ("a", "w", "c"):
             refused(rt, f(**{arg: None}), "null")
         for arg in ("a", "w"):
