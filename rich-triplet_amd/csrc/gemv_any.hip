@@ -32,6 +32,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <atomic>
 
 #include "../../include/rt_hip.h"
@@ -769,14 +770,22 @@ static void any_gateup(const DecodeArgs &a, const LayerArgs &L, int ffn, int K, 
     default: call(RT_LINEAR_Q8_0); break;                         \
   }
 
-static hipError_t any_proj(int fmt, const uint8_t *W, const float *x, float *y, int n, int k, hipStream_t s) {
+static hipError_t any_proj_one(int fmt, const uint8_t *W, const float *x, float *y, int n, int k, hipStream_t s) {
   switch (fmt) {
     case RT_LINEAR_Q6K: return launch_q6k_gemv(W, x, y, n, k, s);
     case RT_LINEAR_Q8_0: return launch_q8_0_gemv(W, x, y, n, k, s);
     case RT_LINEAR_BF16: return launch_bf16_gemv(reinterpret_cast<const uint16_t *>(W), x, y, n, k, s);
-    case RT_LINEAR_MXFP4: return launch_mx_gemv(W, x, y, n, k, s);
     default: return launch_q4k_gemv(W, x, y, n, k, s);
   }
+}
+
+// A set of projections of one input: the MXFP4 ones in one launch, the others one by one.
+static hipError_t any_proj(std::initializer_list<int> fmt, std::initializer_list<const uint8_t *> W, const float *x,
+                           std::initializer_list<float *> y, std::initializer_list<int> n, int k, hipStream_t s) {
+  hipError_t e = launch_mx_set(fmt.begin(), W.begin(), y.begin(), n.begin(), (int)fmt.size(), x, k, s);
+  for (size_t i = 0; i < fmt.size() && e == hipSuccess; ++i)
+    if (fmt.begin()[i] != RT_LINEAR_MXFP4) e = any_proj_one(fmt.begin()[i], W.begin()[i], x, y.begin()[i], n.begin()[i], k, s);
+  return e;
 }
 
 hipError_t enqueue_decode_step_any(const DecodeShape &sh, const DecodeArgs &a, const LayerArgs *layers, hipStream_t s) {
@@ -792,7 +801,7 @@ hipError_t enqueue_decode_step_any(const DecodeShape &sh, const DecodeArgs &a, c
       RT_ANY_FMT(fq, RT_QKV)
 #undef RT_QKV
       ok(hipGetLastError());
-      if (nv == 0) ok(any_proj(fv, L.wv, a.xn, a.v, kvd, H, s));
+      if (nv == 0) ok(any_proj({fv}, {L.wv}, a.xn, {a.v}, {kvd}, H, s));
     } else {
       if (i == 0)
         hipLaunchKernelGGL(k_any_prologue<true>, dim3(1), dim3(512), 0, s, a, nullptr, nullptr, nullptr, L.g_in, H, a.hid,
@@ -801,12 +810,10 @@ hipError_t enqueue_decode_step_any(const DecodeShape &sh, const DecodeArgs &a, c
         hipLaunchKernelGGL(k_any_prologue<false>, dim3(1), dim3(512), 0, s, a, a.x2, a.dn, P.g_post_ffn, L.g_in, H,
                            a.hid, a.xn);
       ok(hipGetLastError());
-      ok(any_proj(fq, L.wq, a.xn, a.q, qd, H, s));
-      ok(any_proj(L.fmt[kProjK], L.wk, a.xn, a.k, kvd, H, s));
-      ok(any_proj(fv, L.wv, a.xn, a.v, kvd, H, s));
+      ok(any_proj({fq, L.fmt[kProjK], fv}, {L.wq, L.wk, L.wv}, a.xn, {a.q, a.k, a.v}, {qd, kvd, kvd}, H, s));
     }
     ok(enqueue_decode_attention(sh, a, L, s));
-    ok(any_proj(L.fmt[kProjO], L.wo, a.attn, a.o, H, qd, s));
+    ok(any_proj({L.fmt[kProjO]}, {L.wo}, a.attn, {a.o}, {H}, qd, s));
     const int fg = L.fmt[kProjGate];
     if (any_set_fmt(fg) && L.fmt[kProjUp] == fg) {
 #define RT_GU(F) any_gateup<F>(a, L, sh.ffn, H, s)
@@ -817,11 +824,10 @@ hipError_t enqueue_decode_step_any(const DecodeShape &sh, const DecodeArgs &a, c
       hipLaunchKernelGGL(k_any_prologue<false>, dim3(1), dim3(512), 0, s, a, a.hid, a.o, L.g_post_attn, L.g_pre_ffn, H,
                          a.x2, a.xn);
       ok(hipGetLastError());
-      ok(any_proj(fg, L.wgate, a.xn, a.h, sh.ffn, H, s));
-      ok(any_proj(L.fmt[kProjUp], L.wup, a.xn, a.u, sh.ffn, H, s));
+      ok(any_proj({fg, L.fmt[kProjUp]}, {L.wgate, L.wup}, a.xn, {a.h, a.u}, {sh.ffn, sh.ffn}, H, s));
       ok(launch_gelu_mul_vec(a.h, a.u, sh.ffn, s));
     }
-    ok(any_proj(L.fmt[kProjDown], L.wdown, a.h, a.dn, H, sh.ffn, s));
+    ok(any_proj({L.fmt[kProjDown]}, {L.wdown}, a.h, {a.dn}, {H}, sh.ffn, s));
     if (e != hipSuccess) return e;
   }
   // final residual and norm (transformer4.rs:2370-2380), then the head

@@ -698,7 +698,10 @@ size_t mx_gemm_workspace_bytes(MxAct act, int m, int n, int k) {
 
 hipError_t launch_mx_gemm(MxAct act, const void *a, const void *w, const float *bias, void *c, bool c_bf16, int m,
                           int n, int k, void *ws, hipStream_t s) {
-  if (mx_rows_ok(act, m, n, k)) return launch_mx_rows(act, a, w, bias, c, c_bf16, m, n, k, ws, s);
+  if (mx_rows_ok(act, m, n, k)) {
+    const MxMat mat{w, c, n};
+    return launch_mx_rows(act, a, &mat, 1, bias, c_bf16, m, k, ws, s);
+  }
   const Plan plan = plan_for(act, m, n, k);
   const int nk = stages_of(plan, k);
   const size_t mk = (size_t)m * k;

@@ -28,12 +28,16 @@ hipError_t launch_mx_gemm(MxAct act, const void *a, const void *w, const float *
 // The same for few rows (mx_rows.hip), which launch_mx_gemm takes where it serves.
 bool mx_rows_ok(MxAct act, int m, int n, int k);
 size_t mx_rows_workspace_bytes(MxAct act, int m, int n, int k);
-// split_done: ws holds this a's digit columns already, from a call with the same act, a, m and k.
-hipError_t launch_mx_rows(MxAct act, const void *a, const void *w, const float *bias, void *c, bool c_bf16, int m,
-                          int n, int k, void *ws, hipStream_t s, bool split_done = false);
-// y = W x of one f32 row; no workspace.
-inline hipError_t launch_mx_gemv(const void *w, const float *x, float *y, int n, int k, hipStream_t s) {
-  return launch_mx_rows(kMxActF32, x, w, nullptr, y, false, 1, n, k, nullptr, s);
-}
+constexpr int kMxSet = 3;  // matrices with the same activations in one launch
+struct MxMat {
+  const void *w;  // planar MXFP4 [n][k]
+  void *c;        // [m][n]
+  int n;
+};
+hipError_t launch_mx_rows(MxAct act, const void *a, const MxMat *mats, int nmat, const float *bias, bool c_bf16,
+                          int m, int k, void *ws, hipStream_t s);
+// y = W x of one f32 row for those of a set's cnt <= kMxSet matrices that are RT_LINEAR_MXFP4; no workspace.
+hipError_t launch_mx_set(const int *fmt, const uint8_t *const *w, float *const *y, const int *n, int cnt,
+                         const float *x, int k, hipStream_t s);
 
 }  // namespace rt

@@ -1,7 +1,8 @@
 // mx_rows.hip -- products of a few rows with an MXFP4 weight: the weight goes
 // from memory to the matrix instructions once, through registers alone.
 //
-// A workgroup owns 16 RT weight rows, its waves share K in pieces (macros) of
+// Up to three matrices with the same activations go in one launch (a step's
+// q|k|v and gate|up).  A workgroup owns 16 RT rows of one of them, its waves share K in pieces (macros) of
 // 512: four instructions, each on 64 bytes of 16 rows and one scale byte per
 // block.  What lies past the end of a row reads as zeros, scale 2^-127.  The
 // activations are the 16 CT columns of the other operand: the digit planes of M
@@ -17,6 +18,7 @@
 
 #include <algorithm>
 
+#include "../../include/rt_hip.h"
 #include "mx_common.hpp"
 #include "mx_digits.hpp"
 #include "mx_kernels.hpp"
@@ -34,12 +36,12 @@ constexpr int digit_area(int cols) { return cols * kPitch + kScaleArea; }  // of
 enum Src { kF32, kBf16, kFp8, kFp4, kCols5, kCols3 };  // kCols: digit columns in fragment order
 
 struct RowsArgs {
-  const uint8_t *w, *wscale;
+  MxMat mat[kMxSet];       // a workgroup is one matrix's: the first `wg[0]` of them mat[0]'s, those below wg[1] mat[1]'s
+  unsigned wg[kMxSet - 1];
   const void *a;           // f32 / bf16 rows, microscaled elements, or digit columns
   const uint8_t *ascale;   // microscaled: [m][K/32]; digit columns: a dword per macro, tile and lane
   const float *bias;
-  void *c;
-  int M, N, K, nmac;
+  int M, K, nmac;
 };
 
 template <int SRC, bool TWO, int RT, int CT, class C>
@@ -49,11 +51,14 @@ __global__ __launch_bounds__(64 * kMaxWaves(RT, CT)) void k_mx_rows(RowsArgs g) 
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = (int)threadIdx.x & 63, l16 = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = (int)blockDim.x >> 6;
-  const int n0 = (int)blockIdx.x * 16 * RT, kb = g.K / 32;
-  const uint8_t *we = g.w + (size_t)n0 * (g.K / 2), *ws = g.wscale + (size_t)n0 * kb;
+  const int in_set = (int)(blockIdx.x >= g.wg[0]) + (int)(blockIdx.x >= g.wg[1]);
+  const MxMat mat = g.mat[in_set];
+  const int N = mat.n, n0 = (int)(blockIdx.x - (in_set ? g.wg[in_set - 1] : 0u)) * 16 * RT, kb = g.K / 32;
+  const uint8_t *we = static_cast<const uint8_t *>(mat.w) + (size_t)n0 * (g.K / 2);
+  const uint8_t *ws = static_cast<const uint8_t *>(mat.w) + (size_t)N * (g.K / 2) + (size_t)n0 * kb;
   int wo[RT];  // this lane's row of each tile
 #pragma unroll
-  for (int i = 0; i < RT; ++i) wo[i] = min(16 * i + l16, g.N - 1 - n0);
+  for (int i = 0; i < RT; ++i) wo[i] = min(16 * i + l16, N - 1 - n0);
   v4f acc[RT][CT];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -167,7 +172,7 @@ __global__ __launch_bounds__(64 * kMaxWaves(RT, CT)) void k_mx_rows(RowsArgs g) 
   __syncthreads();
   for (int o = (int)threadIdx.x; o < 16 * RT * g.M; o += (int)blockDim.x) {
     const int r = o % (16 * RT), m = o / (16 * RT), n = n0 + r;
-    if (n >= g.N) continue;
+    if (n >= N) continue;
     float v = 0.f;
 #pragma unroll 4
     for (int w = 0; w < waves; ++w)
@@ -177,8 +182,8 @@ __global__ __launch_bounds__(64 * kMaxWaves(RT, CT)) void k_mx_rows(RowsArgs g) 
         v += red[(((w * RT + (r >> 4)) * CT + (at >> 4)) * 64 + ((r >> 2) & 3) * 16 + (at & 15)) * 4 + (r & 3)];
       }
     if (g.bias) v += g.bias[n];
-    if constexpr (sizeof(C) == 4) static_cast<float *>(g.c)[(size_t)m * g.N + n] = v;
-    else static_cast<uint16_t *>(g.c)[(size_t)m * g.N + n] = f32_to_bf16_bits(v);
+    if constexpr (sizeof(C) == 4) static_cast<float *>(mat.c)[(size_t)m * N + n] = v;
+    else static_cast<uint16_t *>(mat.c)[(size_t)m * N + n] = f32_to_bf16_bits(v);
   }
 }
 
@@ -247,8 +252,13 @@ auto rows_kernel(const RowsPlan &p) -> void (*)(RowsArgs) {
 }
 
 template <int SRC, bool TWO, class C>
-hipError_t rows_launch(const RowsPlan &p, const RowsArgs &g, hipStream_t s) {
-  const dim3 grid((unsigned)((g.N + 16 * p.rt - 1) / (16 * p.rt))), block(64 * p.waves);
+hipError_t rows_launch(const RowsPlan &p, RowsArgs g, hipStream_t s) {
+  unsigned wgs = 0;
+  for (int i = 0; i < kMxSet; ++i) {
+    wgs += (unsigned)((g.mat[i].n + 16 * p.rt - 1) / (16 * p.rt));
+    if (i < kMxSet - 1) g.wg[i] = wgs;
+  }
+  const dim3 grid(wgs), block(64 * p.waves);
   constexpr int P = SRC == kF32 ? kPlanesF32 : kPlanesBf16;
   const size_t red = (size_t)p.waves * p.rt * p.ct * 1024;
   const size_t dig = SRC == kF32 || SRC == kBf16 ? (size_t)p.waves * digit_area(g.M * P) : 0;
@@ -266,17 +276,20 @@ size_t mx_rows_workspace_bytes(MxAct act, int m, int n, int k) {
   return p.split ? r256(tiles * 8192) + r256(tiles * 256) : 0;
 }
 
-hipError_t launch_mx_rows(MxAct act, const void *a, const void *w, const float *bias, void *c, bool c_bf16, int m,
-                          int n, int k, void *ws, hipStream_t s, bool split_done) {
+hipError_t launch_mx_rows(MxAct act, const void *a, const MxMat *mats, int nmat, const float *bias, bool c_bf16,
+                          int m, int k, void *ws, hipStream_t s) {
+  if (nmat < 1 || nmat > kMxSet) return hipErrorInvalidValue;
+  RowsArgs g{};
+  int n = 0;
+  for (int i = 0; i < nmat; ++i) g.mat[i] = mats[i], n += mats[i].n;
   const RowsPlan p = rows_plan(act, m, n, k);
   const int nmac = (k + kMacro - 1) / kMacro;
-  const uint8_t *we = static_cast<const uint8_t *>(w), *ae = static_cast<const uint8_t *>(a);
-  RowsArgs g{we, we + (size_t)n * k / 2, a, nullptr, bias, c, m, n, k, nmac};
+  const uint8_t *ae = static_cast<const uint8_t *>(a);
+  g.a = a, g.bias = bias, g.M = m, g.K = k, g.nmac = nmac;
   if (p.split) {
     uint8_t *cols = static_cast<uint8_t *>(ws), *sc = cols + r256((size_t)nmac * p.ct * 8192);
     const dim3 grid((unsigned)(((int64_t)m * nmac * (kMacro / 8) + 255) / 256)), block(256);
-    if (split_done) {
-    } else if (act == kMxActF32)
+    if (act == kMxActF32)
       hipLaunchKernelGGL((k_mx_split_cols<float, kPlanesF32>), grid, block, 0, s, static_cast<const float *>(a), cols, sc, m, k, nmac, p.ct);
     else
       hipLaunchKernelGGL((k_mx_split_cols<uint16_t, kPlanesBf16>), grid, block, 0, s, static_cast<const uint16_t *>(a), cols, sc, m, k, nmac, p.ct);
@@ -295,6 +308,15 @@ hipError_t launch_mx_rows(MxAct act, const void *a, const void *w, const float *
       g.ascale = ae + (size_t)m * k / 2;
       return c_bf16 ? rows_launch<kFp4, false, uint16_t>(p, g, s) : rows_launch<kFp4, false, float>(p, g, s);
   }
+}
+
+hipError_t launch_mx_set(const int *fmt, const uint8_t *const *w, float *const *y, const int *n, int cnt,
+                         const float *x, int k, hipStream_t s) {
+  MxMat mats[kMxSet];
+  int nm = 0;
+  for (int i = 0; i < cnt && nm < kMxSet; ++i)
+    if (fmt[i] == RT_LINEAR_MXFP4) mats[nm++] = MxMat{w[i], y[i], n[i]};
+  return nm ? launch_mx_rows(kMxActF32, x, mats, nm, nullptr, false, 1, k, nullptr, s) : hipSuccess;
 }
 
 }  // namespace rt

@@ -865,19 +865,14 @@ hipError_t enqueue_rows(const DecodeShape &s, const DecodeArgs &a, const LayerAr
         for (int c = 0; c < cnt; ++c) *gv[c] = out[c];
         part += (fmt == RT_LINEAR_Q4K ? mb_part_bytes(ntot, K) : kquant_mb_part_bytes(ntot, K)) / sizeof(float);
       }
-      // MXFP4 matrices: from the f32 rows, split into digits once for the set
-      int i = 0;
-      bool split = false;
+      // the MXFP4 matrices in one launch, from the f32 rows
+      MxMat mx[kMxSet];
+      int i = 0, cnt = 0;
       for (const MbMat &m : mats) {
-        if (fmts.begin()[i] == RT_LINEAR_MXFP4) {
-          hipError_t r = launch_mx_rows(kMxActF32, A, m.w, nullptr, m.y, false, n, m.n, K, part, st, split);
-          if (r != hipSuccess) return r;
-          split = true;
-          *views.begin()[i] = rows_plain(m.y, m.n);
-        }
+        if (fmts.begin()[i] == RT_LINEAR_MXFP4) mx[cnt++] = MxMat{m.w, m.y, m.n}, *views.begin()[i] = rows_plain(m.y, m.n);
         ++i;
       }
-      return hipSuccess;
+      return cnt ? launch_mx_rows(kMxActF32, A, mx, cnt, nullptr, false, n, K, part, st) : hipSuccess;
     }
     // A is prepared once for every matrix of the set (q|k|v, gate|up); the
     // norms and the gelu product write it themselves (A == nullptr), at
