@@ -91,11 +91,8 @@ RT_DEV uint32_t buffer_u8(const void *base, int voff, int soff) {
 }
 constexpr int kOutOfRange = (int)0x80000000;
 
-// The elements of 2 and above of four e4m3 bytes (bit 6 is the exponent field's
-// top bit), the others zero.
-RT_DEV uint32_t fp8_upper(uint32_t x) {
-  const uint32_t t = (x >> 6) & 0x01010101u;
-  return x & ((t << 8) - t);
-}
+// Bytes 255 where an e4m3 byte is 2 or more in magnitude (bit 6, the exponent
+// field's top bit, which the permutation spreads as the sign of 16-bit halves), 0 elsewhere.
+RT_DEV uint32_t fp8_upper_mask(uint32_t x) { return __builtin_amdgcn_perm(x << 9, x << 1, 0x090B080Au); }
 
 }  // namespace rt

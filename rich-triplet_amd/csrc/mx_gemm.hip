@@ -103,6 +103,11 @@ RT_DEV uint32_t lds_b32(uint32_t a) {
   asm volatile("ds_read_b32 %0, %1" : "=v"(v) : "v"(a));
   return v;
 }
+RT_DEV uint32_t lds_u8(uint32_t a) {
+  uint32_t v;
+  asm volatile("ds_read_u8 %0, %1" : "=v"(v) : "v"(a));
+  return v;
+}
 RT_DEV uint32_t lds_u16(uint32_t a) {
   uint32_t v;
   asm volatile("ds_read_u16 %0, %1" : "=v"(v) : "v"(a));
@@ -207,7 +212,9 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
   constexpr int kAScale = kWBytes + 512 * ((BN + 127) / 128), kWSlot = kAScale + 512 * ((BM + 127) / 128);
   constexpr int kWCopies = kWBytes / 1024 / kWaves, kACopies = kABytes / 1024 / kWaves;
   static_assert(kWBytes % (1024 * kWaves) == 0 && kABytes % (1024 * kWaves) == 0, "whole copies per wave");
-  constexpr int kALds = 3 * kWSlot, kLds = kALds + 3 * kABytes;
+  // Slots: four, and copies three stages ahead, where two workgroups still share a CU.
+  constexpr int kSlots = BM == 64 ? 4 : 3, kWSlots = P == 1 ? kSlots : 3;
+  constexpr int kALds = kWSlots * kWSlot, kLds = kALds + kSlots * kABytes;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
   const int tid = (int)threadIdx.x, lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
@@ -269,7 +276,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
 #pragma unroll
       for (int i = 0; i < kWCopies; ++i)
         copy_to_lds(wb, base + (kWCopies * wave + i) * 1024, wblk[i] < left ? (int)wo[i] : kOutOfRange, jn * 64);
-      wnext = wnext == 2 ? 0 : wnext + 1;
+      wnext = wnext == kWSlots - 1 ? 0 : wnext + 1;
     }
     const uint8_t *ab = g.a + (size_t)p * g.plane + (size_t)m0 * arow;
 #pragma unroll
@@ -306,7 +313,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
     const uint32_t so = (uint32_t)slot * kWSlot;
 #pragma unroll
     for (int i = 0; i < NT / 4; ++i) f.sw[i] = lds_b32(fws + so + 4 * i);
-    if constexpr (MT == 2) f.sa[0] = lds_u16(fas + so);
+    if constexpr (MT == 1) f.sa[0] = lds_u8(fas + so);
+    else if constexpr (MT == 2) f.sa[0] = lds_u16(fas + so);
     else
 #pragma unroll
       for (int i = 0; i < MT / 4; ++i) f.sa[i] = lds_b32(fas + so + 4 * i);
@@ -347,7 +355,10 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
       v8i up = av;
       if constexpr (TWO) {
 #pragma unroll
-        for (int t = 0; t < 8; ++t) up[t] = (int)fp8_upper((uint32_t)av[t]), av[t] ^= up[t];
+        for (int t = 0; t < 8; ++t) {
+          const uint32_t m = fp8_upper_mask((uint32_t)av[t]);
+          up[t] = (int)((uint32_t)av[t] & m), av[t] = (int)((uint32_t)av[t] & ~m);
+        }
       }
       steps<NT>([&](auto ic) __attribute__((always_inline)) {
         constexpr int i = decltype(ic)::value;
@@ -369,7 +380,10 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
   issue(IntC<0>{}, 0);
   if (n > 1) issue(IntC<1 % P>{}, 1);
   if (n > 2) issue(IntC<2 % P>{}, 2);
-  if (n > 2) wait_vmcnt<copies(1) + copies(2)>();
+  if constexpr (kSlots == 4)
+    if (n > 3) issue(IntC<3 % P>{}, 3);
+  if (kSlots == 4 && n > 3) wait_vmcnt<copies(1) + copies(2) + copies(3)>();
+  else if (n > 2) wait_vmcnt<copies(1) + copies(2)>();
   else if (n > 1) wait_vmcnt<copies(1)>();
   else wait_vmcnt<0>();
   wg_barrier();
@@ -386,15 +400,16 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
       for (int i = 0; i < (MT + 3) / 4; ++i) w.sa[i] -= 0x01010101u * kPlaneShift;  // no borrow: a digit block's byte is at least 20
     done_a(cur);
     if (u + 1 < n) {
-      if (u + 2 < n) wait_vmcnt<copies(p + 2)>();
+      if (kSlots == 4 && u + 3 < n) wait_vmcnt<copies(p + 2) + copies(p + 3)>();
+      else if (u + 2 < n) wait_vmcnt<copies(p + 2)>();
       else wait_vmcnt<0>();
       // every wave has read stage u and has its copies of stage u+1
       wg_barrier();
-      if (u + 3 < n) issue(IntC<(p + 3) % P>{}, slot);
-      slot = slot == 2 ? 0 : slot + 1;
+      if (u + kSlots < n) issue(IntC<(p + kSlots) % P>{}, slot);
+      slot = slot == kSlots - 1 ? 0 : slot + 1;
       read_a(nxt, slot);
       if constexpr ((p + 1) % P == 0) {
-        wslot_r = wslot_r == 2 ? 0 : wslot_r + 1;
+        wslot_r = wslot_r == kWSlots - 1 ? 0 : wslot_r + 1;
         read_w(wn_, wslot_r);
       }
     }
@@ -656,16 +671,31 @@ struct Plan {
   int tile, ksplit;
 };
 // The largest tile that gives every CU one.  Fewer than 256 tiles of 128 x 128:
-// 64 x 128, and K split to about 480 workgroups, which run two or three to a CU
-// (us, 64 x 128 against 128 x 128, each with its best split: 77 x 10240 x 2560 in
-// bf16 20.5 : 22.6, 300 x 2560 x 10240 in MXFP8 31.6 : 34.1, 512 x 2560 x 10240 in
-// f32 72.5 : 72.1).  MXFP4 activations at 4096 x 10240 x 2560: 256 x 256 68 us.
-Plan plan_for(MxAct act, int m, int n, int k) {
+// 64 x 128 (us, against 128 x 128, each with its best split: 77 x 10240 x 2560 in
+// bf16 20.5 : 22.6, 300 x 2560 x 10240 in MXFP8 27.3 : 35.2, 512 x 2560 x 10240 in
+// f32 71.6 : 82.8, 700 x 3840 x 2560 in bf16 34.4 : 37.8).  MXFP4 activations at
+// 4096 x 10240 x 2560: 256 x 256 68 us.
+//
+// K is split where that ends sooner by the times measured (ns): a stage of one
+// plane takes as long beside a second workgroup on its CU as alone (290, of
+// digits 350, of MXFP8 in two instructions 700), 512 workgroups run at once, and
+// the sum costs a launch and every partial value's way out and back.  (300 x
+// 2560 x 2560 in MXFP4: one split 12.4 us, two 14.1, five 17.2; 200 x 2560 x 2560
+// in MXFP8: 17.8, 16.0, 16.2, three 15.3; 100 x 1152 x 6912 in bf16: 57, 36, 20.)
+Plan plan_for(MxAct act, bool c_bf16, int m, int n, int k) {
   auto tiles = [&](int t) { return (int64_t)((m + tile_m(t) - 1) / tile_m(t)) * ((n + tile_n(t) - 1) / tile_n(t)); };
   if (act == kMxActFp4 && tiles(k256x256) >= 256) return {k256x256, 1};
   if (m > 64 && tiles(k128x128) >= 256) return {k128x128, 1};
-  const int64_t ks = std::max<int64_t>(480 / tiles(k64x128), 1);
-  return {k64x128, (int)std::min<int64_t>(ks, (k + 127) / 128)};
+  const int64_t wg = tiles(k64x128), nk = (k + 127) / 128;
+  const double stage = digits(act) ? 350.0 * planes_of(act) : act == kMxActFp8 && !c_bf16 ? 700.0 : 290.0;
+  int best = 1;
+  double best_ns = 0;
+  for (int ks = 1; ks <= nk && ks <= 32; ++ks) {
+    const double run = (double)((wg * ks + 511) / 512) * (double)((nk + ks - 1) / ks) * stage;
+    const double ns = run + (ks > 1 ? 1500.0 + ks * (100.0 + 0.002 * m * n) : 0.0);
+    if (ks == 1 || ns < best_ns) best = ks, best_ns = ns;
+  }
+  return {k64x128, best};
 }
 
 // Stages of 128 of K; in pairs for k256x256.
@@ -681,16 +711,17 @@ hipError_t tile_launch(const TileArgs &g, int tile, hipStream_t s) {
       else hipLaunchKernelGGL((k_mx_gemm_big<C, false>), cus, dim3(256), 0, s, g);
       return hipGetLastError();
     }
-  auto kern = tile == k64x128 ? k_mx_gemm_tile<FA, TWO, P, 2, 2, 4, 2, C> : k_mx_gemm_tile<FA, TWO, P, 2, 2, 4, 4, C>;
+  constexpr bool kOne = FA == kMxFp8 && (TWO || P > 1);
+  auto kern = tile == k64x128 ? k_mx_gemm_tile<FA, TWO, P, kOne ? 1 : 2, kOne ? 4 : 2, kOne ? 8 : 4, kOne ? 1 : 2, C> : k_mx_gemm_tile<FA, TWO, P, 2, 2, 4, 4, C>;
   hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, g);
   return hipGetLastError();
 }
 
 }  // namespace
 
-size_t mx_gemm_workspace_bytes(MxAct act, int m, int n, int k) {
+size_t mx_gemm_workspace_bytes(MxAct act, bool c_bf16, int m, int n, int k) {
   if (mx_rows_ok(act, m, n, k)) return mx_rows_workspace_bytes(act, m, n, k);
-  const Plan p = plan_for(act, m, n, k);
+  const Plan p = plan_for(act, c_bf16, m, n, k);
   const int nk = stages_of(p, k);
   return (digits(act) ? r256((size_t)planes_of(act) * m * k) : 0) + r256(packed_bytes(m, nk)) + r256(packed_bytes(n, nk)) +
          (p.ksplit > 1 ? (size_t)p.ksplit * m * n * 4 : 0);
@@ -702,7 +733,7 @@ hipError_t launch_mx_gemm(MxAct act, const void *a, const void *w, const float *
     const MxMat mat{w, c, n};
     return launch_mx_rows(act, a, &mat, 1, bias, c_bf16, m, k, ws, s);
   }
-  const Plan plan = plan_for(act, m, n, k);
+  const Plan plan = plan_for(act, c_bf16, m, n, k);
   const int nk = stages_of(plan, k);
   const size_t mk = (size_t)m * k;
   uint8_t *p = static_cast<uint8_t *>(ws);

@@ -139,7 +139,10 @@ __global__ __launch_bounds__(64 * kMaxWaves(RT, CT)) void k_mx_rows(RowsArgs g) 
         v8i bv = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]}, up = bv;
         if constexpr (TWO) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) up[i] = (int)fp8_upper((uint32_t)bv[i]), bv[i] ^= up[i];
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t m = fp8_upper_mask((uint32_t)bv[i]);
+            up[i] = (int)((uint32_t)bv[i] & m), bv[i] = (int)((uint32_t)bv[i] & ~m);
+          }
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
