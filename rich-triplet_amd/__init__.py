@@ -255,14 +255,19 @@ def q8_0_gemv(w, x, y, n: int, k: int, stream=None) -> None:
     check(lib().rt_q8_0_gemv(_p(w), _p(x), _p(y), n, k, _stream(stream)))
 
 
+_TORCH_TYPES: dict = {}  # torch dtype -> RT_TYPE_*, filled at the first use
+
+
 def _type(t) -> int:
     """RT_TYPE_* of a torch tensor."""
-    import torch
-    if t.dtype is torch.float32:
-        return TYPE_F32
-    if t.dtype is torch.bfloat16:
-        return TYPE_BF16
-    raise TypeError(f"float32 or bfloat16 wanted, got {t.dtype}")
+    ty = _TORCH_TYPES.get(t.dtype)
+    if ty is None:
+        import torch
+        _TORCH_TYPES.update({torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16})
+        ty = _TORCH_TYPES.get(t.dtype)
+        if ty is None:
+            raise TypeError(f"float32 or bfloat16 wanted, got {t.dtype}")
+    return ty
 
 
 def mx_bytes(fmt: int, rows: int, k: int) -> int:

