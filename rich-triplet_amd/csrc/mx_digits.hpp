@@ -89,6 +89,10 @@ RT_DEV uint32_t buffer_u8(const void *base, int voff, int soff) {
   const auto buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, 0x7FFFFFFF, 0x00020000);
   return (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(buf, voff, soff, 0);
 }
+RT_DEV uint32_t buffer_b32(const void *base, int voff, int soff) {
+  const auto buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, 0x7FFFFFFF, 0x00020000);
+  return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(buf, voff, soff, 0);
+}
 constexpr int kOutOfRange = (int)0x80000000;
 
 // Bytes 255 where an e4m3 byte is 2 or more in magnitude (bit 6, the exponent
