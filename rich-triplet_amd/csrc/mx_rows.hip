@@ -2,15 +2,15 @@
 // from memory to the matrix instructions once, through registers alone.
 //
 // Up to three matrices with the same activations go in one launch (a step's
-// q|k|v and gate|up).  A workgroup owns 16 RT rows of one of them, its waves share K in pieces (macros) of
-// 512: four instructions, each on 64 bytes of 16 rows and one scale byte per
-// block.  What lies past the end of a row reads as zeros, scale 2^-127.  The
-// activations are the 16 CT columns of the other operand: the digit planes of M
-// rows (column m P + p: mx_digits.hpp has the digits), or the rows themselves
-// where they are microscaled.  The
-// waves' sums, and the planes', are added through LDS in a fixed order.
+// q|k|v and gate|up).  A workgroup owns 16 RT rows of one of them, its waves
+// share K in pieces (macros) of 512: four instructions, each on 64 bytes of 16
+// rows and one scale byte per block.  What lies past the end of a row reads as
+// zeros, scale 2^-127.  The activations are the 16 CT columns of the other
+// operand: the digit planes of M rows (column m P + p: mx_digits.hpp has the
+// digits), or the rows themselves where they are microscaled.  The waves' sums,
+// and the planes', are added through LDS in a fixed order.
 //
-// Bound by the weight's bytes: a row of 2560 x 10240 f32 6 to 7 us (2.2 TB/s; a plain
+// Bound by the weight's bytes: one f32 row with 10240 x 2560 6.1 us (2.3 TB/s; a plain
 // streaming read of as many bytes takes 4.2), of which the chain from the row's
 // load over its digits and the instructions to the sum through LDS is what a
 // longer matrix hides; 5 rows x 6912 x 2561 3.1 us for the split and 8.1 us.
