@@ -236,7 +236,8 @@ rt_status rt_gelu_mul_mx(int32_t type, const void *gate, const void *up, int64_t
  * scaled matrix instructions with f32 accumulation: c carries the sum's
  * rounding alone, but that an MXFP8 product into bf16 may lose terms below
  * 2^-13 of the largest of their eight neighbours in k (5e-6 of c's norm).
- * k % 32 == 0, k <= 2^22, m <= 2^30, n <= 2^26; a and w 16-byte aligned.
+ * k % 32 == 0, k <= 2^22, m <= 2^29, n <= 2^26, m n <= 2^35; a and w 16-byte
+ * aligned.
  * Workspace of rt_q4k_gemm_f32: up to (m + n) * k / 32 bytes (each rounded up to
  * whole tiles), plus split-K partials. */
 rt_status rt_mx_gemm(int32_t a_fmt, const void *a, const void *w, const float *bias, int32_t c_type, void *c,

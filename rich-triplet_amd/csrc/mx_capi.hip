@@ -31,8 +31,8 @@ rt_status check_product(const char *who, const void *a, const void *w, const flo
   if (k % kMxBlock != 0) return set_error(RT_EINVAL, "%s: k=%lld must be a multiple of 32", who, (long long)k);
   if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return set_error(RT_EINVAL, "%s: m, n or k exceeds int32", who);
   // 256 rows of either operand stay below 2^31 bytes, a grid's threads below 2^32
-  // (n of a token's product: 16 rows to a workgroup of up to 640)
-  if (k > (1 << 22) || m > (1 << 30) || n > (1 << 26) || m > (int64_t(1) << 38) / n)
+  // (tiles of 64 x 128 in workgroups of 256; few rows: 16 of n in up to 640)
+  if (k > (1 << 22) || m > (1 << 29) || n > (1 << 26) || m > (int64_t(1) << 35) / n)
     return set_error(RT_EINVAL, "%s: m=%lld n=%lld k=%lld is too large", who, (long long)m, (long long)n, (long long)k);
   if (!a || !w || !c) return set_error(RT_EINVAL, "%s: null pointer", who);
   if (!aligned16(a) || !aligned16(w)) return set_error(RT_EINVAL, "%s: a and w must be 16-byte aligned", who);

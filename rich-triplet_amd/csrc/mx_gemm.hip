@@ -212,9 +212,10 @@ RT_DEV void store_tile(const v4f (&acc)[NT][MT], uint8_t *stage, C *c, const flo
 // of MXFP8 elements, which the VALU takes apart), else 32 rows and 64 columns
 // (300 x 2560 x 10240 in MXFP8 27.3 : 29.8 us, 512 x 2560 x 10240 in f32 70.0 : 71.6).
 //
-// Measured: 512 x 2560 x 10240 in f32 61 us, 0.44 us a stage of which the matrix
-// instructions of the CU's two workgroups are 0.23: the stage's chain of barrier,
-// LDS reads and instructions bounds it (with a fourth slot it took as long);
+// Measured: 512 x 2560 x 10240 in f32 59 us, 0.45 us a stage and plane of which the
+// matrix instructions of the CU's workgroups are 0.23 to 0.34: the stage's chain of
+// LDS reads and instructions bounds it, more than its barrier (without it between
+// the planes 1% less) and its copies (a fourth slot: as long);
 // 300 x 2560 x 10240 in MXFP8 19 us; 77 x 10240 x 2560 in bf16 15 us.
 template <int FA, bool TWO, int P, int WN, int WM, int NT, int MT, class C>
 __global__ __launch_bounds__(64 * WN * WM, 2) void k_mx_gemm_tile(TileArgs g) {
@@ -682,11 +683,15 @@ constexpr int tile_n(int t) { return t == k256x256 ? 256 : 128; }
 struct Plan {
   int tile, ksplit;
 };
-// The largest tile that gives every CU one.  Fewer than 256 tiles of 128 x 128:
-// 64 x 128 (us, against 128 x 128, each with its best split: 77 x 10240 x 2560 in
-// bf16 20.4 : 22.6, 300 x 2560 x 10240 in MXFP8 27.4 : 35.2, 512 x 2560 x 10240 in
-// f32 70.5 : 82.8, 700 x 3840 x 2560 in bf16 32.8 : 37.8).  MXFP4 activations at
-// 4096 x 10240 x 2560: 256 x 256 68 us.
+// MXFP4 activations: 256 x 256 where that gives every CU a tile (4096 x 10240 x
+// 2560 68 us).  They and MXFP8 ones in one instruction: else 128 x 128 where that
+// does (us, against 64 x 128: 3000 x 2560 x 10240 in MXFP8 73 : 99, 2048 x 2560 x
+// 10240 in MXFP4 50 : 59).  Digits, MXFP8 in two instructions, and fewer tiles: 64
+// x 128, three workgroups of which share a CU (against 128 x 128, each with its
+// best split: 77 x 10240 x 2560 in bf16 20.4 : 22.6, 300 x 2560 x 10240 in MXFP8
+// 27.4 : 35.2, 4096 x 2560 x 10240 in MXFP8 155 : 195, 512 x 10240 x 2560 in f32
+// 57.9 : 75.1, 4096 x 2560 x 10240 in f32 425 : 492, 4096 x 10240 x 2560 in bf16
+// 246 : 241, in f32 the same).
 //
 // K is split where that ends sooner by the times measured (ns): a stage of one
 // plane takes 290, of digits 350, of MXFP8 in two instructions 700, nearly as
@@ -698,9 +703,10 @@ struct Plan {
 Plan plan_for(MxAct act, bool c_bf16, int m, int n, int k) {
   auto tiles = [&](int t) { return (int64_t)((m + tile_m(t) - 1) / tile_m(t)) * ((n + tile_n(t) - 1) / tile_n(t)); };
   if (act == kMxActFp4 && tiles(k256x256) >= 256) return {k256x256, 1};
-  if (m > 64 && tiles(k128x128) >= 256) return {k128x128, 1};
+  const bool two = act == kMxActFp8 && !c_bf16;
+  if (!digits(act) && !two && m > 64 && tiles(k128x128) >= 256) return {k128x128, 1};
   const int64_t wg = tiles(k64x128), nk = (k + 127) / 128;
-  const double stage = digits(act) ? 350.0 * planes_of(act) : act == kMxActFp8 && !c_bf16 ? 700.0 : 290.0;
+  const double stage = digits(act) ? 350.0 * planes_of(act) : two ? 700.0 : 290.0;
   auto load = [](int64_t w) { return w == 0 ? 0.0 : w <= 256 ? 1.0 : w <= 512 ? 1.05 : 1.3; };  // w workgroups on 256 CUs
   int best = 1;
   double best_ns = 0;
@@ -725,9 +731,12 @@ hipError_t tile_launch(const TileArgs &g, int tile, hipStream_t s) {
       else hipLaunchKernelGGL((k_mx_gemm_big<C, false>), cus, dim3(256), 0, s, g);
       return hipGetLastError();
     }
-  constexpr bool kOne = FA == kMxFp8 && (TWO || P > 1);
-  auto kern = tile == k64x128 ? k_mx_gemm_tile<FA, TWO, P, kOne ? 1 : 2, kOne ? 4 : 2, kOne ? 8 : 4, kOne ? 1 : 2, C> : k_mx_gemm_tile<FA, TWO, P, 2, 2, 4, 4, C>;
-  hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, g);
+  if constexpr (TWO || P > 1) {
+    hipLaunchKernelGGL((k_mx_gemm_tile<FA, TWO, P, 1, 4, 8, 1, C>), grid, dim3(256), 0, s, g);
+  } else {
+    auto kern = tile == k64x128 ? k_mx_gemm_tile<FA, false, 1, 2, 2, 4, 2, C> : k_mx_gemm_tile<FA, false, 1, 2, 2, 4, 4, C>;
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, g);
+  }
   return hipGetLastError();
 }
 

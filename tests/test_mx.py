@@ -174,6 +174,9 @@ def test_products_refuse_before_launch(rt, ptr):
         refused(rt, f(n=1 << 31), "int32")
         refused(rt, f(n=1 << 27), "too large")  # a grid's threads pass 2^32
         refused(rt, f(k=1 << 23), "too large")
+        if name not in ("gemv", "batch"):
+            refused(rt, f(m=1 << 30), "too large")
+            refused(rt, f(m=1 << 20, n=1 << 16), "too large")
         for arg in ("a", "w", "c"):
             refused(rt, f(**{arg: None}), "null")
         for arg in ("a", "w"):
